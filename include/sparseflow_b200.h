@@ -327,6 +327,65 @@ SFB200_API int sfb200_debug_route_gemm(int M, int N, int K, int swiglu, int num_
 SFB200_API int sfb200_debug_host_pipeline(int main_rows, int tail_rows);
 SFB200_API int sfb200_debug_host_chunk_plan(int M, int main_rows, int tail_rows, int* out8);
 
+/* ------------------------------------------------------------------ 1b. around the FFN ------ */
+/* Operators that stand next to the gated FFN: a mixture of experts over 2:4 weights (router, products grouped by expert,
+ * weighted sum), the norms between two blocks, and low-rank adapters beside a projection.  No counterpart upstream.
+ * Everything is decided on the device (group sizes are never read by the host), so each call can be captured into a graph. */
+
+/* Device scratch of sfb200_group_rows above 4096 entries and of sfb200_moe_route above 64 tokens, for that many groups
+ * (experts); below, workspace may be NULL. */
+SFB200_API size_t sfb200_group_workspace_bytes(int groups);
+
+/* Groups n entries by id: offsets[groups + 1] = entries of the groups before each, slots[n] = place of an entry in the order
+ * (group, entry), -1 for an id outside 0 .. groups-1, rows[n] = entry / per_row of every place, -1 behind the last group.
+ * 1 <= groups <= 1024. */
+SFB200_API int sfb200_group_rows(const int* ids, int n, int groups, int per_row, int* offsets, int* rows, int* slots,
+                                 void* workspace, void* stream);
+
+/* Router: chosen[tokens, top_k] = the top_k largest logits of a token, largest first, ties to the lowest expert;
+ * weights = their softmax over all experts (renormalize: over the chosen ones).  A logit of -inf or NaN is never chosen: where fewer
+ * than top_k are left, chosen is -1 and the weight 0.  +inf counts as the largest finite number.  offsets, rows, slots: the
+ * grouping of the entries by expert with per_row = top_k, so rows holds tokens.  dtype: sfb200_dtype, or 2 for float logits.
+ * experts <= 1024, top_k <= 32 and <= experts. */
+SFB200_API int sfb200_moe_route(const void* logits, int64_t ld, int tokens, int experts, int top_k, int dtype, int renormalize,
+                                float* weights, int* chosen, int* offsets, int* rows, int* slots, void* workspace, void* stream);
+
+/* y[p] = act(W_e . x[p] + bias[e]) for offsets[e] <= p < offsets[e + 1], W_e [N, K] 2:4-compressed, the experts' values and
+ * metadata one after the other (metadata padded to whole tiles per expert).  rows != NULL: x[rows[p]] in place of x[p], x_rows rows
+ * of x (gathered: scratch of total * K elements).  Places behind offsets[experts] are left as they were.  total: rows of y (with rows
+ * NULL also of x).  K % 64 == 0, N % 8 == 0, pitches % 8 == 0, 16-byte aligned, experts <= 1024. */
+SFB200_API int sfb200_grouped_sparse_gemm(const void* x, int ldx, int x_rows, const int* rows, void* gathered, const void* values,
+                                          const void* meta, void* y, int ldy, int total, int experts, int N, int K, int dtype,
+                                          const void* bias, int act, const int* offsets, void* stream);
+/* h[p] = silu(Wg_e . x + gate_bias[e]) * (Wu_e . x + up_bias[e]): every expert's 2 * I rows in the order of
+ * sfb200_prune_compress_gate_up.  I % 16 == 0. */
+SFB200_API int sfb200_grouped_sparse_gemm_swiglu(const void* x, int ldx, int x_rows, const int* rows, void* gathered,
+                                                 const void* values_gu, const void* meta_gu, void* h, int ldh, int total, int experts,
+                                                 int I, int K, int dtype, const void* gate_bias, const void* up_bias,
+                                                 const int* offsets, void* stream);
+
+/* out[t] = residual[t] + sum_j weights[t, j] * y[slots[t, j]]; residual may be NULL; a slot outside 0 .. y_rows-1 adds nothing.
+ * 32-bit sums in the order of j. */
+SFB200_API int sfb200_moe_combine(const void* y, int64_t ld_y, int y_rows, const int* slots, const float* weights, const void* residual,
+                                  int64_t ld_res, void* out, int64_t ld_out, int tokens, int top_k, int cols, int dtype, void* stream);
+
+/* Between two blocks: r = x + scale * gate * z with z = y or norm(y) * post_weight + post_bias, and h = norm(r) * weight + bias of
+ * the unrounded r.  norm: rms (layer = 0) or layer norm.  y NULL: h = norm(x) only (r, gate, post_* NULL).  h may be NULL.
+ * gate [gate_rows, gate_cols]: gate_cols = cols or 1, every gate row serves rows / gate_rows consecutive rows.  Types: sfb200_dtype or 2
+ * (float); x and r have x_type, everything else y_type; x_type equals y_type or is float.  cols <= 16384.  r may be x, h may be y. */
+SFB200_API int sfb200_block_norm(const void* x, int64_t ld_x, const void* y, int64_t ld_y, const void* weight, const void* bias,
+                                 const void* post_weight, const void* post_bias, const void* gate, int64_t ld_gate, int gate_rows,
+                                 int gate_cols, void* r, int64_t ld_r, void* h, int64_t ld_h, int rows, int cols, int x_type, int y_type,
+                                 float scale, float eps, float post_eps, int layer, void* stream);
+
+SFB200_API size_t sfb200_lora_workspace_bytes(int n, int rank);
+/* out[t] = y[t] + scales[g] * (x[t] . A_g^T) . B_g^T for the rows of group g (grouping with per_row = 1 over n rows); rows of no
+ * group: out[t] = y[t].  a [groups, rank, K], b [groups, N, rank] contiguous, rank 8, 16, 32, 64 or 128 (pad with zeros), K and N
+ * multiples of 8, pitches % 8 == 0, 16-byte aligned, groups <= 1024.  out may be y. */
+SFB200_API int sfb200_lora_add(const void* y, int64_t ld_y, const void* x, int64_t ld_x, const void* a, const void* b, const float* scales,
+                               void* out, int64_t ld_out, int n, int groups, int rank, int K, int N, int dtype, const int* offsets,
+                               const int* rows, const int* slots, void* workspace, void* stream);
+
 /* ------------------------------------------------------------------ 2. sf_* runtime API --- */
 /* experiments/old_structure/runtime/api/sparseflow_api.h:8-28, exercised by tests/test_c_api.cpp. */
 

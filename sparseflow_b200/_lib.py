@@ -83,6 +83,18 @@ def lib() -> C.CDLL:
     L.sfb200_sparse_gemm_f32out.argtypes = [vp, i, vp, vp, vp, i, i, i, i, i, vp, i, vp]
     L.sfb200_ffn_forward_noalloc.argtypes = [C.POINTER(FFNWeights), vp, i, vp, i, i, vp]
     L.sfb200_noalloc_device_status.argtypes = [C.POINTER(C.c_int)]
+    i64, f = C.c_int64, C.c_float
+    L.sfb200_group_workspace_bytes.restype = sz
+    L.sfb200_group_workspace_bytes.argtypes = [i]
+    L.sfb200_group_rows.argtypes = [vp, i, i, i, vp, vp, vp, vp, vp]
+    L.sfb200_moe_route.argtypes = [vp, i64, i, i, i, i, i, vp, vp, vp, vp, vp, vp, vp]
+    L.sfb200_grouped_sparse_gemm.argtypes = [vp, i, i, vp, vp, vp, vp, vp, i, i, i, i, i, i, vp, i, vp, vp]
+    L.sfb200_grouped_sparse_gemm_swiglu.argtypes = [vp, i, i, vp, vp, vp, vp, vp, i, i, i, i, i, i, vp, vp, vp, vp]
+    L.sfb200_moe_combine.argtypes = [vp, i64, i, vp, vp, vp, i64, vp, i64, i, i, i, i, vp]
+    L.sfb200_block_norm.argtypes = [vp, i64, vp, i64, vp, vp, vp, vp, vp, i64, i, i, vp, i64, vp, i64, i, i, i, i, f, f, f, i, vp]
+    L.sfb200_lora_workspace_bytes.restype = sz
+    L.sfb200_lora_workspace_bytes.argtypes = [i, i]
+    L.sfb200_lora_add.argtypes = [vp, i64, vp, i64, vp, vp, vp, vp, i64, i, i, i, i, i, i, vp, vp, vp, vp, vp]
     L.sfb200_debug_wait_timeout.argtypes = [C.c_uint, i, i, vp]
     L.sf_select_kernel.restype = C.c_int32
     L.sf_select_kernel.argtypes = [C.c_char_p, C.POINTER(MatmulDesc), C.POINTER(GpuInfo)]

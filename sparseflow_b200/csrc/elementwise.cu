@@ -10,6 +10,7 @@
 
 #include "kernels.h"
 #include "launch.h"
+#include "row_divider.h"
 #include "sm100_ptx.cuh"
 
 namespace sfb200 {
@@ -43,18 +44,6 @@ __device__ __forceinline__ uint32_t silu_mul2(uint32_t g2, uint32_t u2) {
 // with a 64-bit division per piece the kernel ran at 4.8 TB/s, and with one block per 2048 columns of a row 64-wide pitched
 // rows left 248 of 256 threads idle.  16384 x 64 / 262144 x 64 pitched: 2.8 / 21.9 us with the division, 17.4 / 77.7 us with blocks of
 // columns, now 2.4 / 17.8 us; unpitched 262144 x 64 17.1 us.
-struct RowDivider {
-  uint64_t mul;
-  int shift;
-};
-// For 1 <= d <= 2^28 and 0 <= i < 2^31: i / d == i * mul >> shift, with l = ceil(log2 d), shift = 31 + l and
-// mul = floor(2^shift / d) + 1: 2^shift < mul * d <= 2^shift + 2^l, so the product is above i / d by less than
-// i * 2^l / (d * 2^shift) < 1 / d.  mul <= 2^32: the product fits 64 bits.
-RowDivider row_divider(uint32_t d) {
-  int l = 0;
-  while ((1ull << l) < d) ++l;
-  return RowDivider{(1ull << (31 + l)) / d + 1, 31 + l};
-}
 template <bool BF16>
 __global__ void __launch_bounds__(256) silu_mul_vec_kernel(const uint16_t* g, const uint16_t* u, uint16_t* o, uint32_t pieces,
                                                            uint32_t row_pieces, RowDivider div, int ldg, int ldu, int ldo) {

@@ -149,4 +149,82 @@ constexpr int kSmallMMaxTokens = 4;
 int launch_silu_mul(const void* gate, const void* up, void* out, int rows, int cols, int ld_g,
                     int ld_u, int ld_o, int fmt, cudaStream_t stream);
 
+// ---- operators around the gated FFN ------------------------------------------------------------
+// Grouping of entries by id (ids outside 0 .. groups-1: no group).  workspace: group_workspace_bytes(groups).
+struct GroupArgs {
+  const int* ids;
+  int n, groups, per_row;
+  int *offsets, *rows, *slots;      // [groups + 1], [n], [n]
+  void* workspace;
+};
+int launch_group_rows(const GroupArgs& a, cudaStream_t stream);
+size_t group_workspace_bytes(int groups);
+// Router: top_k of every token's logits, weights, and the grouping of the tokens by expert.
+struct RouteArgs {
+  const void* logits;      // [tokens, experts], row pitch ld
+  int64_t ld;
+  int tokens, experts, top_k;
+  int dtype;               // 0 f16, 1 bf16, 2 f32
+  int renorm;
+  float* weights;          // [tokens, top_k]
+  int* chosen;             // [tokens, top_k]
+  int *offsets, *rows, *slots;
+  void* workspace;
+};
+int launch_moe_route(const RouteArgs& a, cudaStream_t stream);
+// out[t] = residual[t] + sum_j weights[t, j] * y[slots[t, j]]
+struct CombineArgs {
+  const void* y;
+  int64_t ld_y;
+  int y_rows;
+  const int* slots;
+  const float* weights;
+  const void* residual;    // or null
+  int64_t ld_res;
+  void* out;
+  int64_t ld_out;
+  int tokens, top_k, cols, fmt;
+};
+int launch_moe_combine(const CombineArgs& a, cudaStream_t stream);
+// Between two blocks: r = x + scale * gate * post(y), h = norm(r).
+struct NormArgs {
+  const void *x, *y;       // y or null (then r, gate and post_* are null)
+  const void *weight, *bias, *post_weight, *post_bias, *gate;
+  void *r, *h;             // either may be null
+  int64_t ld_x, ld_y, ld_r, ld_h, ld_gate;
+  int rows, cols, gate_rows, gate_cols;      // gate [gate_rows, gate_cols], gate_cols 1 or cols
+  int x_type, y_type;      // 0 f16, 1 bf16, 2 f32: x and r; everything else.  Equal, or x_type 2
+  float scale, eps, post_eps;
+  int layer;               // 0 rms, 1 layer norm
+};
+constexpr int kNormMaxCols = 16384;
+int launch_block_norm(const NormArgs& a, cudaStream_t stream);
+// out = y + scales[g] * (x . A_g^T) . B_g^T by the rows' groups.  workspace: n * rank floats.
+struct LoraArgs {
+  const void *y, *x, *a, *b;      // [n, N], [n, K], [groups, rank, K], [groups, N, rank]
+  const float* scales;
+  void* out;
+  const int *offsets, *rows, *slots;
+  void* workspace;
+  int64_t ld_y, ld_x, ld_out;
+  int n, groups, rank, K, N, fmt;
+};
+int launch_lora_add(const LoraArgs& a, cudaStream_t stream);
+// Sparse GEMM grouped by expert: rows offsets[e] .. offsets[e+1] of y through weight e.
+struct GroupedGemmArgs {
+  const void* x;           // [x_rows, K], row pitch ldx, in the order of the groups
+  const void* values;      // [experts, n_out, K/2]
+  const void* meta;        // tiled metadata of every expert, one after the other
+  const void* bias;        // as GroupedParams
+  const void* bias_up;
+  const int* offsets;
+  void* y;
+  int* status;
+  int x_rows, total;       // total: rows of y (the groups fill at most these)
+  int experts, n_out, K, ldx, ldy, fmt, epi, act, num_sms;
+};
+int launch_grouped_gemm(const GroupedGemmArgs& a, cudaStream_t stream);
+// dst[i] = src[rows[i]] (zeros where rows[i] is outside 0 .. src_rows-1), cols % 8 == 0
+int launch_gather_rows(const void* src, int64_t ld, int src_rows, const int* rows, int n, int cols, void* dst, cudaStream_t stream);
+
 }  // namespace sfb200

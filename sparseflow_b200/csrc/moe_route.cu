@@ -1,0 +1,317 @@
+// Grouping of rows, and the router of a mixture of experts.
+//
+// Grouping: entries 0 .. n-1 carry the id of a group (or none); offsets[g] counts the entries of the groups before g, and the
+// entries of a group keep their order, so that the place of an entry is
+//   slots[i] = offsets[id_i] + |{i' < i : id_i' = id_i}|,   rows[slots[i]] = i / per_row.
+// Integer counts only: the same result on every run.
+//
+// Router: p = softmax(l_t); the top_k largest logits of a token, ties to the lowest expert, with their p (or p over the sum of the
+// chosen).  An expert whose logit is -inf or NaN is never chosen; a token with fewer than top_k others gets expert -1, weight 0
+// there, and belongs to no group (rows of padding: all logits -inf).  +inf counts as the largest finite number.
+//
+// One warp works on one token: a lane keeps the logits of experts lane, lane + 32, ... as unsigned keys that order like the
+// numbers, and top_k rounds take the largest key and, among equals, the lowest expert (two warp reductions a round).
+// Work is latency: 16 bytes a chosen entry and one pass over the logits are 1 us of HBM time at 8192 x 128.  Blocks own runs
+// of consecutive tokens; with one block everything is a single launch, otherwise a second launch adds up the
+// blocks' counts (at most kMaxBlocks x groups) and places the entries.
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+#include <float.h>
+#include <stdint.h>
+
+#include "kernels.h"
+#include "launch.h"
+#include "sm100_ptx.cuh"
+
+namespace sfb200 {
+namespace {
+
+constexpr int kThreads = 512, kWarps = kThreads / 32, kMaxBlocks = 128, kMaxGroups = 1024;
+
+struct GroupParams {
+  const int* ids;      // [n]: the caller's, or the experts that the router wrote
+  int n;               // entries
+  int groups;
+  int per_row;         // entries per row
+  int chunk;           // entries per block
+  int* counts;         // [blocks][groups], two launches only
+  int* offsets;        // [groups + 1]
+  int* rows;           // [n]
+  int* slots;          // [n]
+};
+struct RouteParams {
+  const void* logits;
+  int64_t ld;
+  int tokens, experts, top_k, dtype, renorm, tokens_per_block;
+  float* weights;      // [tokens, top_k]
+  int* chosen;         // [tokens, top_k]
+};
+
+__device__ __forceinline__ int entry_group(const GroupParams& p, int i, int end) {
+  if (i >= end) return -1;
+  const int id = p.ids[i];
+  return id >= 0 && id < p.groups ? id : -1;
+}
+
+// The chunk's entries per group into hist[groups].
+__device__ void count_chunk(const GroupParams& p, int begin, int end, int* hist) {
+  for (int g = threadIdx.x; g < p.groups; g += kThreads) hist[g] = 0;
+  __syncthreads();
+  for (int i0 = begin; i0 < end; i0 += kThreads) {
+    const int g = entry_group(p, i0 + threadIdx.x, end);
+    const unsigned same = __match_any_sync(0xffffffffu, g);
+    if (g >= 0 && __ffs(same) - 1 == (threadIdx.x & 31)) atomicAdd(&hist[g], __popc(same));
+  }
+  __syncthreads();
+}
+
+// total[g] -> exclusive prefix sums in base[g]; returns the sum of all.  groups <= 1024: two per thread.
+__device__ int scan_groups(int groups, const int* total, int* base) {
+  __shared__ int warp_sum[kWarps];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g0 = 2 * threadIdx.x;
+  const int a = g0 < groups ? total[g0] : 0, b = g0 + 1 < groups ? total[g0 + 1] : 0;
+  int v = a + b;
+#pragma unroll
+  for (int d = 1; d < 32; d <<= 1) {
+    const int u = __shfl_up_sync(0xffffffffu, v, d);
+    if (lane >= d) v += u;
+  }
+  if (lane == 31) warp_sum[warp] = v;
+  __syncthreads();
+  int before = 0, all = 0;
+#pragma unroll
+  for (int w = 0; w < kWarps; ++w) {
+    const int s = warp_sum[w];
+    if (w < warp) before += s;
+    all += s;
+  }
+  const int first = before + v - a - b;
+  if (g0 < groups) base[g0] = first;
+  if (g0 + 1 < groups) base[g0 + 1] = first + a;
+  __syncthreads();
+  return all;
+}
+
+// Places the chunk's entries: base[g] is the place of the chunk's first entry of group g; wcnt is scratch.
+__device__ void place_chunk(const GroupParams& p, int begin, int end, int* base, uint16_t* wcnt) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  for (int i0 = begin; i0 < end; i0 += kThreads) {
+    for (int j = threadIdx.x; j < kWarps * p.groups; j += kThreads) wcnt[j] = 0;
+    __syncthreads();
+    const int i = i0 + threadIdx.x, g = entry_group(p, i, end);
+    const unsigned same = __match_any_sync(0xffffffffu, g);
+    const int rank = __popc(same & ((1u << lane) - 1u));
+    if (g >= 0 && rank == 0) wcnt[warp * p.groups + g] = static_cast<uint16_t>(__popc(same));
+    __syncthreads();
+    for (int e = threadIdx.x; e < p.groups; e += kThreads) {      // counts of the warps before, at most kThreads
+      int run = 0;
+#pragma unroll
+      for (int w = 0; w < kWarps; ++w) {
+        const int c = wcnt[w * p.groups + e];
+        wcnt[w * p.groups + e] = static_cast<uint16_t>(run);
+        run += c;
+      }
+    }
+    __syncthreads();
+    if (i < end) {
+      int at = -1;
+      if (g >= 0) {
+        at = base[g] + wcnt[warp * p.groups + g] + rank;
+        p.rows[at] = i / p.per_row;
+      }
+      p.slots[i] = at;
+    }
+    __syncthreads();
+    if (g >= 0) {      // the last warp that has an entry of this group carries its base on
+      if (rank == 0) atomicAdd(&base[g], __popc(same));
+    }
+    __syncthreads();
+  }
+}
+
+__device__ __forceinline__ uint32_t order_key(float v) {
+  if (!(v > -INFINITY)) return 0;                 // -inf and NaN: never chosen
+  const uint32_t u = __float_as_uint(fminf(v, FLT_MAX));
+  return u ^ ((u >> 31) ? 0xffffffffu : 0x80000000u);
+}
+__device__ __forceinline__ float key_value(uint32_t k) {
+  return __uint_as_float(k ^ ((k >> 31) ? 0x80000000u : 0xffffffffu));
+}
+__device__ __forceinline__ float warp_sum(float v) {
+#pragma unroll
+  for (int d = 16; d > 0; d >>= 1) v += __shfl_xor_sync(0xffffffffu, v, d);
+  return v;
+}
+
+// NL: logits per lane
+template <int NL>
+__device__ void route_tokens(const RouteParams& r, int t_begin, int t_end) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  for (int t = t_begin + warp; t < t_end; t += kWarps) {
+    uint32_t key[NL];
+#pragma unroll
+    for (int i = 0; i < NL; ++i) {
+      const int e = i * 32 + lane;
+      float v = -INFINITY;
+      if (e < r.experts) {
+        const int64_t at = t * r.ld + e;
+        if (r.dtype == 2) v = static_cast<const float*>(r.logits)[at];
+        else if (r.dtype == kBF16) v = __bfloat162float(static_cast<const __nv_bfloat16*>(r.logits)[at]);
+        else v = __half2float(static_cast<const __half*>(r.logits)[at]);
+      }
+      key[i] = order_key(v);
+    }
+    float largest = 0.f, everyone = 0.f, mine = 0.f;      // lane j keeps the j-th choice
+    int expert = -1;
+    for (int j = 0; j < r.top_k; ++j) {
+      uint32_t k = 0;
+      int e = 0x7fffffff;
+#pragma unroll
+      for (int i = 0; i < NL; ++i)
+        if (key[i] > k) { k = key[i]; e = i * 32 + lane; }
+      const uint32_t top = __reduce_max_sync(0xffffffffu, k);
+      if (top == 0) break;
+      e = static_cast<int>(__reduce_min_sync(0xffffffffu, k == top ? static_cast<unsigned>(e) : 0x7fffffffu));
+      const float v = key_value(top);
+      if (j == 0) {
+        largest = v;
+        if (!r.renorm) {
+#pragma unroll
+          for (int i = 0; i < NL; ++i)
+            if (key[i] != 0) everyone += expf(key_value(key[i]) - v);
+          everyone = warp_sum(everyone);
+        }
+      }
+      if (lane == j) { expert = e; mine = expf(v - largest); }
+#pragma unroll
+      for (int i = 0; i < NL; ++i)
+        if (i * 32 + lane == e) key[i] = 0;
+    }
+    if (r.renorm) everyone = warp_sum(mine);
+    if (lane < r.top_k) {
+      const int64_t at = static_cast<int64_t>(t) * r.top_k + lane;
+      r.weights[at] = expert >= 0 ? mine / everyone : 0.f;
+      r.chosen[at] = expert;
+    }
+  }
+}
+
+// NL = 0: the ids are the caller's.  ONE: a single block does everything; otherwise this launch leaves the blocks' counts.
+template <int NL, bool ONE>
+__global__ void __launch_bounds__(kThreads) group_kernel(const RouteParams r, const GroupParams p) {
+  __shared__ int base[kMaxGroups], hist[kMaxGroups];
+  __shared__ uint16_t wcnt[ONE ? kWarps * kMaxGroups : 1];
+  dependency_wait();
+  dependency_trigger();
+  const int64_t begin64 = static_cast<int64_t>(blockIdx.x) * p.chunk;
+  const int begin = static_cast<int>(begin64 < p.n ? begin64 : p.n);
+  const int end = begin64 + p.chunk < p.n ? begin + p.chunk : p.n;
+  if (NL > 0) {
+    const int t0 = blockIdx.x * r.tokens_per_block;
+    const int t1 = t0 + r.tokens_per_block < r.tokens ? t0 + r.tokens_per_block : r.tokens;
+    route_tokens<NL == 0 ? 1 : NL>(r, t0, t1);
+    __syncthreads();
+  }
+  count_chunk(p, begin, end, hist);
+  if (ONE) {
+    const int all = scan_groups(p.groups, hist, base);
+    for (int g = threadIdx.x; g < p.groups; g += kThreads) p.offsets[g] = base[g];
+    if (threadIdx.x == 0) p.offsets[p.groups] = all;
+    for (int i = all + threadIdx.x; i < p.n; i += kThreads) p.rows[i] = -1;
+    __syncthreads();
+    place_chunk(p, begin, end, base, wcnt);
+  } else {
+    for (int g = threadIdx.x; g < p.groups; g += kThreads) p.counts[static_cast<size_t>(blockIdx.x) * p.groups + g] = hist[g];
+  }
+}
+
+__global__ void __launch_bounds__(kThreads) place_kernel(const GroupParams p) {
+  __shared__ int base[kMaxGroups], total[kMaxGroups];
+  __shared__ uint16_t wcnt[kWarps * kMaxGroups];
+  dependency_wait();
+  dependency_trigger();
+  const int me = blockIdx.x;
+  int before[(kMaxGroups + kThreads - 1) / kThreads];
+#pragma unroll
+  for (int j = 0; j < kMaxGroups / kThreads; ++j) {
+    const int g = threadIdx.x + j * kThreads;
+    int sum = 0, pre = 0;
+    if (g < p.groups) {
+#pragma unroll 8
+      for (int b = 0; b < static_cast<int>(gridDim.x); ++b) {
+        const int c = p.counts[static_cast<size_t>(b) * p.groups + g];
+        sum += c;
+        pre += b < me ? c : 0;
+      }
+      total[g] = sum;
+    }
+    before[j] = pre;
+  }
+  __syncthreads();
+  const int all = scan_groups(p.groups, total, base);
+  if (me == 0) {
+    for (int g = threadIdx.x; g < p.groups; g += kThreads) p.offsets[g] = base[g];
+    if (threadIdx.x == 0) p.offsets[p.groups] = all;
+    __syncthreads();
+  }
+#pragma unroll
+  for (int j = 0; j < kMaxGroups / kThreads; ++j) {
+    const int g = threadIdx.x + j * kThreads;
+    if (g < p.groups) base[g] += before[j];
+  }
+  __syncthreads();
+  const int64_t begin64 = static_cast<int64_t>(me) * p.chunk;
+  const int begin = static_cast<int>(begin64 < p.n ? begin64 : p.n);
+  const int end = begin64 + p.chunk < p.n ? begin + p.chunk : p.n;
+  for (int i = (begin > all ? begin : all) + threadIdx.x; i < end; i += kThreads) p.rows[i] = -1;      // behind the last group
+  place_chunk(p, begin, end, base, wcnt);
+}
+
+template <int NL>
+int launch_group(const RouteParams& r, const GroupParams& p, int blocks, cudaStream_t stream) {
+  if (blocks == 1) return launch_dependent(group_kernel<NL, true>, 1, kThreads, 0, 0, stream, r, p);
+  const int rc = launch_dependent(group_kernel<NL, false>, blocks, kThreads, 0, 0, stream, r, p);
+  if (rc != kOk) return rc;
+  return launch_dependent(place_kernel, blocks, kThreads, 0, 0, stream, p);
+}
+
+}  // namespace
+
+size_t group_workspace_bytes(int groups) { return static_cast<size_t>(kMaxBlocks) * groups * sizeof(int); }
+
+int launch_group_rows(const GroupArgs& a, cudaStream_t stream) {
+  if (a.n < 0 || a.groups < 1 || a.groups > kMaxGroups || a.per_row < 1 || !a.offsets) return kErrInvalid;
+  if (a.n > 0 && (!a.ids || !a.rows || !a.slots)) return kErrInvalid;
+  GroupParams p{a.ids, a.n, a.groups, a.per_row, 0, static_cast<int*>(a.workspace), a.offsets, a.rows, a.slots};
+  // one block to 4096 entries: eight rounds of 512 cost less than a second launch
+  const int blocks = a.n <= 4096 ? 1 : kMaxBlocks;
+  if (blocks > 1 && !a.workspace) return kErrInvalid;
+  p.chunk = blocks == 1 ? a.n : (a.n + blocks - 1) / blocks;
+  return launch_group<0>(RouteParams{}, p, blocks, stream);
+}
+
+int launch_moe_route(const RouteArgs& a, cudaStream_t stream) {
+  if (a.tokens < 0 || a.experts < 1 || a.experts > kMaxGroups || a.top_k < 1 || a.top_k > 32 || a.top_k > a.experts) return kErrInvalid;
+  if (a.dtype < 0 || a.dtype > 2 || a.ld < a.experts || !a.offsets) return kErrInvalid;
+  if (a.tokens > 0 && (!a.logits || !a.weights || !a.chosen || !a.rows || !a.slots)) return kErrInvalid;
+  if (static_cast<int64_t>(a.tokens) * a.top_k > 0x7fffffffll - kThreads) return kErrInvalid;
+  const int n = a.tokens * a.top_k;
+  // to 64 tokens one block (four tokens a warp) costs less than a second launch; beyond, 16 tokens a block or more
+  int per_block = a.tokens;
+  if (a.tokens > 64) {
+    per_block = (a.tokens + kMaxBlocks - 1) / kMaxBlocks;
+    if (per_block < kWarps) per_block = kWarps;
+  }
+  const int blocks = a.tokens > 0 ? (a.tokens + per_block - 1) / per_block : 1;
+  if (blocks > 1 && !a.workspace) return kErrInvalid;
+  const RouteParams r{a.logits, a.ld, a.tokens, a.experts, a.top_k, a.dtype, a.renorm, per_block, a.weights, a.chosen};
+  const GroupParams p{a.chosen, n, a.experts, a.top_k, per_block * a.top_k, static_cast<int*>(a.workspace), a.offsets, a.rows, a.slots};
+  if (a.experts <= 32) return launch_group<1>(r, p, blocks, stream);
+  if (a.experts <= 64) return launch_group<2>(r, p, blocks, stream);
+  if (a.experts <= 128) return launch_group<4>(r, p, blocks, stream);
+  if (a.experts <= 256) return launch_group<8>(r, p, blocks, stream);
+  return launch_group<32>(r, p, blocks, stream);
+}
+
+}  // namespace sfb200
