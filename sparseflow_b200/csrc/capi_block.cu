@@ -26,13 +26,12 @@ int sfb200_moe_route(const void* logits, int64_t ld, int tokens, int experts, in
                           static_cast<cudaStream_t>(stream));
 }
 
-static int grouped(const void* x, int ldx, int x_rows, const int* rows, void* gathered, const void* values, const void* meta, void* y, int ldy,
+static int grouped(const void* x, int ldx, int x_rows, const int* rows, const void* values, const void* meta, void* y, int ldy,
                    int total, int experts, int N, int K, int dtype, const void* bias, const void* bias_up, int act, int epi, const int* offsets,
                    void* stream) {
   int err = kOk;
   DeviceState* s = device_state(&err);
   if (!s) return err;
-  cudaStream_t st = static_cast<cudaStream_t>(stream);
   GroupedGemmArgs a{};
   a.x = x;
   a.values = values;
@@ -40,6 +39,7 @@ static int grouped(const void* x, int ldx, int x_rows, const int* rows, void* ga
   a.bias = bias;
   a.bias_up = bias_up;
   a.offsets = offsets;
+  a.rows = rows;
   a.y = y;
   a.status = s->status;
   a.x_rows = x_rows;
@@ -53,27 +53,19 @@ static int grouped(const void* x, int ldx, int x_rows, const int* rows, void* ga
   a.epi = epi;
   a.act = act;
   a.num_sms = s->num_sms;
-  if (rows != nullptr && total > 0) {
-    if (!gathered || !x || ldx < K || ldx % 8 != 0 || K % 8 != 0) return kErrInvalid;
-    const int rc = launch_gather_rows(x, ldx, x_rows, rows, total, K, gathered, st);
-    if (rc != kOk) return rc;
-    a.x = gathered;
-    a.ldx = K;
-    a.x_rows = total;
-  }
-  return launch_grouped_gemm(a, st);
+  return launch_grouped_gemm(a, static_cast<cudaStream_t>(stream));
 }
 
-int sfb200_grouped_sparse_gemm(const void* x, int ldx, int x_rows, const int* rows, void* gathered, const void* values, const void* meta, void* y,
+int sfb200_grouped_sparse_gemm(const void* x, int ldx, int x_rows, const int* rows, const void* values, const void* meta, void* y,
                                int ldy, int total, int experts, int N, int K, int dtype, const void* bias, int act, const int* offsets, void* stream) {
-  return grouped(x, ldx, x_rows, rows, gathered, values, meta, y, ldy, total, experts, N, K, dtype, bias, nullptr, act, kEpiStore, offsets, stream);
+  return grouped(x, ldx, x_rows, rows, values, meta, y, ldy, total, experts, N, K, dtype, bias, nullptr, act, kEpiStore, offsets, stream);
 }
 
-int sfb200_grouped_sparse_gemm_swiglu(const void* x, int ldx, int x_rows, const int* rows, void* gathered, const void* values_gu, const void* meta_gu,
+int sfb200_grouped_sparse_gemm_swiglu(const void* x, int ldx, int x_rows, const int* rows, const void* values_gu, const void* meta_gu,
                                       void* h, int ldh, int total, int experts, int I, int K, int dtype, const void* gate_bias, const void* up_bias,
                                       const int* offsets, void* stream) {
   if (I <= 0 || I > 0x3fffffff) return kErrInvalid;
-  return grouped(x, ldx, x_rows, rows, gathered, values_gu, meta_gu, h, ldh, total, experts, 2 * I, K, dtype, gate_bias, up_bias, kActNone, kEpiSwiGLU,
+  return grouped(x, ldx, x_rows, rows, values_gu, meta_gu, h, ldh, total, experts, 2 * I, K, dtype, gate_bias, up_bias, kActNone, kEpiSwiGLU,
                  offsets, stream);
 }
 

@@ -19,9 +19,10 @@ struct GroupedParams {
   const void* bias;       // store: [experts, n_out]; SiLU.mul: gate rows, [experts, n_out / 2]; or null
   const void* bias_up;    // SiLU.mul: up rows, or null
   const int* offsets;     // [experts + 1]
+  const int* rows;        // [total]: row of x for every place, or null (x is in the order of the places)
   void* y;
   int* status;
-  int experts, n_out, K, ldy, total;
+  int experts, n_out, K, ldy, total, x_rows;
   int row_tiles;          // metadata tiles of 128 rows per expert
   int k_tiles128;
   int m_blks;             // row tiles of the kernel per expert
@@ -34,6 +35,8 @@ inline GroupedParams grouped_params(const GroupedGemmArgs& a) {
   p.bias = a.bias;
   p.bias_up = a.bias_up;
   p.offsets = a.offsets;
+  p.rows = a.rows;
+  p.x_rows = a.x_rows;
   p.y = a.y;
   p.status = a.status;
   p.experts = a.experts;
@@ -100,6 +103,32 @@ __device__ __forceinline__ void locate_tile(const GroupedParams& p, int bn, cons
   t.tok0 = first_row[t.e] + b * each;
   const int left = n - b * each;
   t.count = left < each ? left : each;
+}
+
+// Four rows of a token operand into 4 x 128 bytes of a swizzled tile, by one copy (box of one row).  The pair form credits the bytes to the
+// barrier of the pair's even CTA.
+__device__ __forceinline__ void tma_gather4(uint32_t dst, const CUtensorMap* m, int x, const int (&r)[4], uint32_t bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.shared::cta.global.tile::gather4.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5, %6}], [%7];" ::"r"(dst),
+      "l"(reinterpret_cast<uint64_t>(m)), "r"(x), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(bar)
+      : "memory");
+}
+__device__ __forceinline__ void tma_gather4_pair(uint32_t dst, const CUtensorMap* m, int x, const int (&r)[4], uint32_t leader_bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.shared::cluster.global.tile::gather4.mbarrier::complete_tx::bytes.cta_group::2 [%0], [%1, {%2, %3, %4, %5, %6}], "
+      "[%7];" ::"r"(dst),
+      "l"(reinterpret_cast<uint64_t>(m)), "r"(x), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(leader_bar)
+      : "memory");
+}
+// The four rows of x that a lane fetches: places first + 4 * lane .. of a run of `count` (a lane behind its end: nothing).
+__device__ __forceinline__ void gather_rows_of(const GroupedParams& p, int first, int count, int (&r)[4]) {
+  const int lane = threadIdx.x & 31;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    int i = 4 * lane + j;
+    if (i >= count) i = count - 1;
+    r[j] = count > 0 ? min(max(p.rows[first + i], 0), p.x_rows - 1) : 0;
+  }
 }
 
 // 16-token chunks [c_begin, c_end) of a warp's 32 accumulator lanes (rows row_w ..): load, convert, transpose through the staging

@@ -212,7 +212,8 @@ struct LoraArgs {
 int launch_lora_add(const LoraArgs& a, cudaStream_t stream);
 // Sparse GEMM grouped by expert: rows offsets[e] .. offsets[e+1] of y through weight e.
 struct GroupedGemmArgs {
-  const void* x;           // [x_rows, K], row pitch ldx, in the order of the groups
+  const void* x;           // [x_rows, K], row pitch ldx: a row per place, or read through rows
+  const int* rows;         // [total] row of x for every place, or null
   const void* values;      // [experts, n_out, K/2]
   const void* meta;        // tiled metadata of every expert, one after the other
   const void* bias;        // as GroupedParams
@@ -224,7 +225,7 @@ struct GroupedGemmArgs {
   int experts, n_out, K, ldx, ldy, fmt, epi, act, num_sms;
 };
 int launch_grouped_gemm(const GroupedGemmArgs& a, cudaStream_t stream);
-// dst[i] = src[rows[i]] (zeros where rows[i] is outside 0 .. src_rows-1), cols % 8 == 0
-int launch_gather_rows(const void* src, int64_t ld, int src_rows, const int* rows, int n, int cols, void* dst, cudaStream_t stream);
+// The CTA-pair form of it, for many tokens per expert.
+int launch_grouped_gemm_pair(const GroupedGemmArgs& a, cudaStream_t stream);
 
 }  // namespace sfb200

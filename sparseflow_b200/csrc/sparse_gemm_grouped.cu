@@ -29,9 +29,10 @@
 namespace sfb200 {
 namespace {
 
-template <int BN_, int STAGES_, int EPI_>
+template <int BN_, int STAGES_, int EPI_, bool GATHER_>
 struct GCfg {
   static constexpr int BN = BN_, STAGES = STAGES_, EPI = EPI_;
+  static constexpr bool GATHER = GATHER_;      // token rows fetched four by four through p.rows
   static constexpr int BK = 128;
   static constexpr int A_BYTES = 128 * 64 * 2;
   static constexpr int B_SUB_BYTES = BN * 128;
@@ -49,7 +50,7 @@ struct GCfg {
   static constexpr int OFF_BAR = OFF_D + D_BYTES;
   static constexpr int OFF_TABLE = OFF_BAR + 256;
   static constexpr int SMEM_BYTES = OFF_TABLE + 1024;      // + the tables of tiles, sized at launch, + alignment slack
-  static_assert(BN % 16 == 0 && BN >= 32 && BN <= 128, "BN");
+  static_assert(BN % 16 == 0 && BN >= 32 && BN <= 128, "BN: at most four rows per producer lane");
   static_assert(8 * (2 * STAGES + 4) + 8 <= 256, "barriers");
 };
 
@@ -101,27 +102,44 @@ grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
   const int num_tiles = first_tile[p.experts];
 
   if (warp == 0) {
-    if (elect_one()) {
-      int s = 0;
-      uint32_t ph = 0;
-      bool ok = true;
-      GroupedTile t;
-      t.e = 0;
-      for (int tile = blockIdx.x; tile < num_tiles && ok; tile += gridDim.x) {
-        locate_tile(p, C::BN, first_tile, first_row, tile, t);
-        const uint32_t* meta = p.meta + (static_cast<size_t>(t.e) * p.row_tiles + t.m_blk) * p.k_tiles128 * 512;
-        for (int kt = 0; kt < k_iters; ++kt) {
-          ok = mbar_wait(bar_empty + 8 * s, ph ^ 1, err, p.status, 1);
-          if (!ok) break;
-          const uint32_t full = bar_full + 8 * s;
-          mbar_arrive_expect_tx(full, C::A_BYTES + C::B_BYTES + C::E_BYTES);
+    // TMA producer: one lane waits, announces the bytes and copies the weight; the token tile is one box by the same lane, or
+    // four rows per lane
+    const bool one = elect_one();
+    int s = 0;
+    uint32_t ph = 0;
+    bool ok = true;
+    GroupedTile t;
+    t.e = 0;
+    for (int tile = blockIdx.x; tile < num_tiles && ok; tile += gridDim.x) {
+      locate_tile(p, C::BN, first_tile, first_row, tile, t);
+      const uint32_t* meta = p.meta + (static_cast<size_t>(t.e) * p.row_tiles + t.m_blk) * p.k_tiles128 * 512;
+      const int fours = (t.count + 3) / 4;
+      int rows[4];
+      if (C::GATHER) gather_rows_of(p, t.tok0, t.count, rows);
+      const uint32_t b_bytes = C::GATHER ? static_cast<uint32_t>(fours) * 1024u : C::B_BYTES;
+      for (int kt = 0; kt < k_iters; ++kt) {
+        ok = mbar_wait(bar_empty + 8 * s, ph ^ 1, err, p.status, 1);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        const uint32_t full = bar_full + 8 * s;
+        const uint32_t b_dst = sbase + C::OFF_B + s * C::B_BYTES;
+        if (one) {
+          mbar_arrive_expect_tx(full, C::A_BYTES + C::E_BYTES + b_bytes);
           tma_load_2d(sbase + C::OFF_A + s * C::A_BYTES, &tmA, kt * 64, t.e * p.n_out + t.m_blk * 128, full);
-#pragma unroll
-          for (int j = 0; j < 2; ++j)
-            tma_load_2d(sbase + C::OFF_B + s * C::B_BYTES + j * C::B_SUB_BYTES, &tmB, kt * C::BK + j * 64, t.tok0, full);
           bulk_load_1d(sbase + C::OFF_E + s * C::E_BYTES, meta + static_cast<size_t>(kt) * 512, C::E_BYTES, full);
-          if (++s == C::STAGES) { s = 0; ph ^= 1; }
+          if (!C::GATHER) {
+#pragma unroll
+            for (int j = 0; j < 2; ++j) tma_load_2d(b_dst + j * C::B_SUB_BYTES, &tmB, kt * C::BK + j * 64, t.tok0, full);
+          }
         }
+        if (C::GATHER) {
+          __syncwarp();      // the bytes are announced before any arrive
+          if (lane < fours) {
+#pragma unroll
+            for (int j = 0; j < 2; ++j) tma_gather4(b_dst + j * C::B_SUB_BYTES + lane * 512, &tmB, kt * C::BK + j * 64, rows, full);
+          }
+        }
+        if (++s == C::STAGES) { s = 0; ph ^= 1; }
       }
     }
   } else if (warp == 1) {
@@ -196,19 +214,6 @@ grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
   }
 }
 
-__global__ void __launch_bounds__(256) gather_rows_kernel(const uint16_t* src, int64_t ld, int src_rows, const int* rows, int n, int pieces, uint16_t* dst) {
-  dependency_wait();
-  dependency_trigger();
-  for (int i = blockIdx.x; i < n; i += gridDim.x) {
-    const int r = rows[i];
-    const bool ok = r >= 0 && r < src_rows;
-    for (int c = threadIdx.x; c < pieces; c += 256) {
-      const uint4 v = ok ? *reinterpret_cast<const uint4*>(src + r * ld + c * 8) : make_uint4(0, 0, 0, 0);
-      *reinterpret_cast<uint4*>(dst + (static_cast<size_t>(i) * pieces + c) * 8) = v;
-    }
-  }
-}
-
 template <class C>
 int launch_cfg(const GroupedGemmArgs& a, cudaStream_t stream) {
   const int smem = C::SMEM_BYTES + (2 * (a.experts + 1) * 4 + 15) / 16 * 16;
@@ -225,26 +230,20 @@ int launch_cfg(const GroupedGemmArgs& a, cudaStream_t stream) {
   const uint64_t kc = static_cast<uint64_t>(a.K) / 2;
   if (!make_map_2d(&tmA, a.values, static_cast<uint64_t>(a.experts) * a.n_out, kc, kc * 2, 128, 64, CU_TENSOR_MAP_SWIZZLE_128B, a.fmt))
     return kErrTensorMap;
-  if (!make_map_2d(&tmB, a.x, a.x_rows, a.K, static_cast<uint64_t>(a.ldx) * 2, C::BN, 64, CU_TENSOR_MAP_SWIZZLE_128B, a.fmt)) return kErrTensorMap;
+  if (!make_map_2d(&tmB, a.x, a.x_rows, a.K, static_cast<uint64_t>(a.ldx) * 2, C::GATHER ? 1 : C::BN, 64, CU_TENSOR_MAP_SWIZZLE_128B, a.fmt)) return kErrTensorMap;
   const GroupedParams p = grouped_params(a);
   return launch_dependent(grouped_gemm_kernel<C>, a.num_sms, 192, smem, 0, stream, tmA, tmB, p);
 }
 
-template <int EPI>
+template <int EPI, bool GATHER>
 int dispatch(const GroupedGemmArgs& a, cudaStream_t stream) {
   const int per_expert = a.total / a.experts;
-  if (per_expert <= 24) return launch_cfg<GCfg<32, 7, EPI>>(a, stream);
-  if (per_expert <= 64) return launch_cfg<GCfg<64, 6, EPI>>(a, stream);
-  return launch_cfg<GCfg<128, 4, EPI>>(a, stream);
+  if (per_expert <= 24) return launch_cfg<GCfg<32, 7, EPI, GATHER>>(a, stream);
+  if (per_expert <= 64) return launch_cfg<GCfg<64, 6, EPI, GATHER>>(a, stream);
+  return launch_grouped_gemm_pair(a, stream);
 }
 
 }  // namespace
-
-int launch_gather_rows(const void* src, int64_t ld, int src_rows, const int* rows, int n, int cols, void* dst, cudaStream_t stream) {
-  if (n <= 0) return kOk;
-  return launch_dependent(gather_rows_kernel, n < 148 * 16 ? n : 148 * 16, 256, 0, 0, stream, static_cast<const uint16_t*>(src), ld, src_rows, rows, n,
-                          cols / 8, static_cast<uint16_t*>(dst));
-}
 
 int launch_grouped_gemm(const GroupedGemmArgs& a, cudaStream_t stream) {
   if (a.experts < 1 || a.experts > kMaxExperts || a.total < 0 || a.K <= 0 || a.K % 64 != 0 || a.n_out <= 0 || a.n_out % 8 != 0) return kErrInvalid;
@@ -261,9 +260,9 @@ int launch_grouped_gemm(const GroupedGemmArgs& a, cudaStream_t stream) {
   if (static_cast<int64_t>((a.n_out + 127) / 128) * (a.total / 16 + a.experts) > 0x7fffffffll) return kErrInvalid;
   if (a.epi == kEpiSwiGLU) {
     if (a.n_out % 32 != 0) return kErrInvalid;
-    return dispatch<kEpiSwiGLU>(a, stream);
+    return a.rows ? dispatch<kEpiSwiGLU, true>(a, stream) : dispatch<kEpiSwiGLU, false>(a, stream);
   }
-  return dispatch<kEpiStore>(a, stream);
+  return a.rows ? dispatch<kEpiStore, true>(a, stream) : dispatch<kEpiStore, false>(a, stream);
 }
 
 }  // namespace sfb200

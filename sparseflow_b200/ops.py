@@ -512,8 +512,7 @@ def grouped_sparse_gemm(x: torch.Tensor, cw: CompressedExperts, groups: RowGroup
             _check_out(out, x, (total, cw.rows), x.dtype)
         if total == 0:
             return out
-        scratch = x.new_empty((total, cw.K)) if gather else None
-        rc = _lib.lib().sfb200_grouped_sparse_gemm(x.data_ptr(), _pitch(x), x.shape[0], groups.rows.data_ptr() if gather else None, _ptr(scratch),
+        rc = _lib.lib().sfb200_grouped_sparse_gemm(x.data_ptr(), _pitch(x), x.shape[0], groups.rows.data_ptr() if gather else None,
                                                    cw.values.data_ptr(), cw.meta.data_ptr(), out.data_ptr(), _pitch(out), total, cw.experts, cw.rows,
                                                    cw.K, _dt(x), _ptr(bias), ACT[act], groups.offsets.data_ptr(), _stream())
     if rc:
@@ -539,9 +538,8 @@ def grouped_sparse_gemm_swiglu(x: torch.Tensor, cw_gu: CompressedExperts, groups
             _check_out(out, x, (total, I), x.dtype)
         if total == 0:
             return out
-        scratch = x.new_empty((total, cw_gu.K)) if gather else None
         rc = _lib.lib().sfb200_grouped_sparse_gemm_swiglu(x.data_ptr(), _pitch(x), x.shape[0], groups.rows.data_ptr() if gather else None,
-                                                          _ptr(scratch), cw_gu.values.data_ptr(), cw_gu.meta.data_ptr(), out.data_ptr(), _pitch(out),
+                                                          cw_gu.values.data_ptr(), cw_gu.meta.data_ptr(), out.data_ptr(), _pitch(out),
                                                           total, cw_gu.experts, I, cw_gu.K, _dt(x), _ptr(gate_bias), _ptr(up_bias),
                                                           groups.offsets.data_ptr(), _stream())
     if rc:
