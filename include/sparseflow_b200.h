@@ -352,14 +352,15 @@ SFB200_API int sfb200_moe_route(const void* logits, int64_t ld, int tokens, int 
 
 /* y[p] = act(W_e . x[p] + bias[e]) for offsets[e] <= p < offsets[e + 1], W_e [N, K] 2:4-compressed, the experts' values and
  * metadata one after the other (metadata padded to whole tiles per expert).  rows != NULL: x[rows[p]] in place of x[p], x_rows rows
- * of x.  Places behind offsets[experts] are left as they were.  total: rows of y (with rows
+ * of x, and scratch of sfb200_grouped_scratch_bytes (may be NULL where that is 0).  Places behind offsets[experts] are left as they were.  total: rows of y (with rows
  * NULL also of x).  K % 64 == 0, N % 8 == 0, pitches % 8 == 0, 16-byte aligned, experts <= 1024. */
-SFB200_API int sfb200_grouped_sparse_gemm(const void* x, int ldx, int x_rows, const int* rows, const void* values,
+SFB200_API int sfb200_grouped_sparse_gemm(const void* x, int ldx, int x_rows, const int* rows, void* scratch, const void* values,
                                           const void* meta, void* y, int ldy, int total, int experts, int N, int K, int dtype,
                                           const void* bias, int act, const int* offsets, void* stream);
+SFB200_API size_t sfb200_grouped_scratch_bytes(int total, int experts, int N, int K);
 /* h[p] = silu(Wg_e . x + gate_bias[e]) * (Wu_e . x + up_bias[e]): every expert's 2 * I rows in the order of
  * sfb200_prune_compress_gate_up.  I % 16 == 0. */
-SFB200_API int sfb200_grouped_sparse_gemm_swiglu(const void* x, int ldx, int x_rows, const int* rows,
+SFB200_API int sfb200_grouped_sparse_gemm_swiglu(const void* x, int ldx, int x_rows, const int* rows, void* scratch,
                                                  const void* values_gu, const void* meta_gu, void* h, int ldh, int total, int experts,
                                                  int I, int K, int dtype, const void* gate_bias, const void* up_bias,
                                                  const int* offsets, void* stream);

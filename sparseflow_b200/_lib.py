@@ -88,8 +88,12 @@ def lib() -> C.CDLL:
     L.sfb200_group_workspace_bytes.argtypes = [i]
     L.sfb200_group_rows.argtypes = [vp, i, i, i, vp, vp, vp, vp, vp]
     L.sfb200_moe_route.argtypes = [vp, i64, i, i, i, i, i, vp, vp, vp, vp, vp, vp, vp]
-    L.sfb200_grouped_sparse_gemm.argtypes = [vp, i, i, vp, vp, vp, vp, i, i, i, i, i, i, vp, i, vp, vp]
-    L.sfb200_grouped_sparse_gemm_swiglu.argtypes = [vp, i, i, vp, vp, vp, vp, i, i, i, i, i, i, vp, vp, vp, vp]
+    L.sfb200_grouped_scratch_bytes.restype = sz
+    L.sfb200_grouped_scratch_bytes.argtypes = [i, i, i, i]
+    L.sfb200_debug_plan_grouped.argtypes = [i, i, i, i, i, i]
+    L.sfb200_debug_force_grouped.argtypes = [i]
+    L.sfb200_grouped_sparse_gemm.argtypes = [vp, i, i, vp, vp, vp, vp, vp, i, i, i, i, i, i, vp, i, vp, vp]
+    L.sfb200_grouped_sparse_gemm_swiglu.argtypes = [vp, i, i, vp, vp, vp, vp, vp, i, i, i, i, i, i, vp, vp, vp, vp]
     L.sfb200_moe_combine.argtypes = [vp, i64, i, vp, vp, vp, i64, vp, i64, i, i, i, i, vp]
     L.sfb200_block_norm.argtypes = [vp, i64, vp, i64, vp, vp, vp, vp, vp, i64, i, i, vp, i64, vp, i64, i, i, i, i, f, f, f, i, vp]
     L.sfb200_lora_workspace_bytes.restype = sz

@@ -26,7 +26,7 @@ int sfb200_moe_route(const void* logits, int64_t ld, int tokens, int experts, in
                           static_cast<cudaStream_t>(stream));
 }
 
-static int grouped(const void* x, int ldx, int x_rows, const int* rows, const void* values, const void* meta, void* y, int ldy,
+static int grouped(const void* x, int ldx, int x_rows, const int* rows, void* scratch, const void* values, const void* meta, void* y, int ldy,
                    int total, int experts, int N, int K, int dtype, const void* bias, const void* bias_up, int act, int epi, const int* offsets,
                    void* stream) {
   int err = kOk;
@@ -40,6 +40,8 @@ static int grouped(const void* x, int ldx, int x_rows, const int* rows, const vo
   a.bias_up = bias_up;
   a.offsets = offsets;
   a.rows = rows;
+  a.scratch = scratch;
+  a.variant = s->force_grouped;
   a.y = y;
   a.status = s->status;
   a.x_rows = x_rows;
@@ -56,16 +58,40 @@ static int grouped(const void* x, int ldx, int x_rows, const int* rows, const vo
   return launch_grouped_gemm(a, static_cast<cudaStream_t>(stream));
 }
 
-int sfb200_grouped_sparse_gemm(const void* x, int ldx, int x_rows, const int* rows, const void* values, const void* meta, void* y,
-                               int ldy, int total, int experts, int N, int K, int dtype, const void* bias, int act, const int* offsets, void* stream) {
-  return grouped(x, ldx, x_rows, rows, values, meta, y, ldy, total, experts, N, K, dtype, bias, nullptr, act, kEpiStore, offsets, stream);
+size_t sfb200_grouped_scratch_bytes(int total, int experts, int N, int K) {
+  int err = kOk;
+  DeviceState* s = device_state(&err);
+  if (!s || total <= 0 || experts <= 0 || N <= 0 || K <= 0) return 0;
+  const int variant = s->force_grouped ? s->force_grouped : plan_grouped(total, experts, N, K, true, s->num_sms);
+  return variant >= 10000 ? static_cast<size_t>(total) * K * 2 : 0;
 }
 
-int sfb200_grouped_sparse_gemm_swiglu(const void* x, int ldx, int x_rows, const int* rows, const void* values_gu, const void* meta_gu,
+/* Which form a grouped product over `total` places runs on a GPU with num_sms SMs: 32 / 64 single-CTA tiles of that many tokens; 1128, 1240 /
+ * 2128, 2240 CTA-pair tiles of 256 / 512 rows; 10000 more: rows copied into the order of the experts first.  Host-only. */
+SFB200_API int sfb200_debug_plan_grouped(int total, int experts, int N, int K, int gather, int num_sms) {
+  if (total <= 0 || experts <= 0 || N <= 0 || K <= 0 || num_sms <= 0) return 0;
+  return plan_grouped(total, experts, N, K, gather != 0, num_sms);
+}
+
+/* Test hook: force the form of grouped products (0 = automatic). */
+SFB200_API int sfb200_debug_force_grouped(int variant) {
+  int err = kOk;
+  DeviceState* s = device_state(&err);
+  if (!s) return err;
+  s->force_grouped = variant;
+  return kOk;
+}
+
+int sfb200_grouped_sparse_gemm(const void* x, int ldx, int x_rows, const int* rows, void* scratch, const void* values, const void* meta, void* y,
+                               int ldy, int total, int experts, int N, int K, int dtype, const void* bias, int act, const int* offsets, void* stream) {
+  return grouped(x, ldx, x_rows, rows, scratch, values, meta, y, ldy, total, experts, N, K, dtype, bias, nullptr, act, kEpiStore, offsets, stream);
+}
+
+int sfb200_grouped_sparse_gemm_swiglu(const void* x, int ldx, int x_rows, const int* rows, void* scratch, const void* values_gu, const void* meta_gu,
                                       void* h, int ldh, int total, int experts, int I, int K, int dtype, const void* gate_bias, const void* up_bias,
                                       const int* offsets, void* stream) {
   if (I <= 0 || I > 0x3fffffff) return kErrInvalid;
-  return grouped(x, ldx, x_rows, rows, values_gu, meta_gu, h, ldh, total, experts, 2 * I, K, dtype, gate_bias, up_bias, kActNone, kEpiSwiGLU,
+  return grouped(x, ldx, x_rows, rows, scratch, values_gu, meta_gu, h, ldh, total, experts, 2 * I, K, dtype, gate_bias, up_bias, kActNone, kEpiSwiGLU,
                  offsets, stream);
 }
 

@@ -16,6 +16,7 @@ struct DeviceState {
   size_t total_mem = 0;
   int* status = nullptr;       // device status word (256-byte allocation, word 0 used)
   int force_bn = 0;            // tuning hook: token tile override
+  int force_grouped = 0;       // test hook: form of the grouped products
   void* stage_x = nullptr;     // host-buffer FFN: device copies of x / out, hidden scratch
   void* stage_o = nullptr;
   void* stage_h = nullptr;

@@ -105,8 +105,8 @@ __device__ __forceinline__ void locate_tile(const GroupedParams& p, int bn, cons
   t.count = left < each ? left : each;
 }
 
-// Four rows of a token operand into 4 x 128 bytes of a swizzled tile, by one copy (box of one row).  The pair form credits the bytes to the
-// barrier of the pair's even CTA.
+// Four rows of a token operand into 4 x 128 bytes of a swizzled tile, by one copy (box of one row).  The pair form credits the bytes to
+// the barrier of the pair's even CTA.
 __device__ __forceinline__ void tma_gather4(uint32_t dst, const CUtensorMap* m, int x, const int (&r)[4], uint32_t bar) {
   asm volatile(
       "cp.async.bulk.tensor.2d.shared::cta.global.tile::gather4.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5, %6}], [%7];" ::"r"(dst),
@@ -120,12 +120,11 @@ __device__ __forceinline__ void tma_gather4_pair(uint32_t dst, const CUtensorMap
       "l"(reinterpret_cast<uint64_t>(m)), "r"(x), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(leader_bar)
       : "memory");
 }
-// The four rows of x that a lane fetches: places first + 4 * lane .. of a run of `count` (a lane behind its end: nothing).
-__device__ __forceinline__ void gather_rows_of(const GroupedParams& p, int first, int count, int (&r)[4]) {
-  const int lane = threadIdx.x & 31;
+// The four rows of x that copy number `at` fetches: places first + 4 * at .. of a run of `count`.
+__device__ __forceinline__ void gather_rows_of(const GroupedParams& p, int first, int count, int at, int (&r)[4]) {
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
-    int i = 4 * lane + j;
+    int i = 4 * at + j;
     if (i >= count) i = count - 1;
     r[j] = count > 0 ? min(max(p.rows[first + i], 0), p.x_rows - 1) : 0;
   }
@@ -160,22 +159,26 @@ __device__ __forceinline__ void drain_tile(const GroupedParams& p, const Grouped
   auto store_chunk = [&](const uint32_t* a, const uint32_t* b, int c) {
     const uint32_t stage = stage0 + (c & buf_mask) * D_BUF_BYTES;
     __syncwarp();
+    // which conversion runs is tested once per chunk, not once per value: the drain is a chain of dependent instructions
     if (EPI == kEpiSwiGLU) {
-      if (gate_up_bias) {
-        auto f = [&](int i, float bg, float bu) { return silu_mul_bias(a[i], b[i], bg, bu); };
-        stmatrix_x4_trans(stage + st_off, pack16(f(0, b0, b2), f(1, b0, b2), p.fmt), pack16(f(2, b1, b3), f(3, b1, b3), p.fmt),
-                          pack16(f(4, b0, b2), f(5, b0, b2), p.fmt), pack16(f(6, b1, b3), f(7, b1, b3), p.fmt));
-      } else {
-        stmatrix_x4_trans(stage + st_off, pack16(silu_mul(a[0], b[0]), silu_mul(a[1], b[1]), p.fmt),
-                          pack16(silu_mul(a[2], b[2]), silu_mul(a[3], b[3]), p.fmt), pack16(silu_mul(a[4], b[4]), silu_mul(a[5], b[5]), p.fmt),
-                          pack16(silu_mul(a[6], b[6]), silu_mul(a[7], b[7]), p.fmt));
-      }
+      auto emit = [&](auto f, const int fmt) {
+        stmatrix_x4_trans(stage + st_off, pack16(f(0, b0, b2), f(1, b0, b2), fmt), pack16(f(2, b1, b3), f(3, b1, b3), fmt),
+                          pack16(f(4, b0, b2), f(5, b0, b2), fmt), pack16(f(6, b1, b3), f(7, b1, b3), fmt));
+      };
+      if (gate_up_bias) emit([&](int i, float bg, float bu) { return silu_mul_bias(a[i], b[i], bg, bu); }, p.fmt);
+      else if (p.fmt == kBF16) emit([&](int i, float, float) { return silu_mul(a[i], b[i]); }, kBF16);
+      else emit([&](int i, float, float) { return silu_mul(a[i], b[i]); }, kF16);
     } else {
-      auto f = [&](uint32_t v, float bias) { return act_fn(__uint_as_float(v) + bias, p.act); };
-      stmatrix_x4_trans(stage + st_off, pack16(f(a[0], b0), f(a[1], b0), p.fmt), pack16(f(a[2], b1), f(a[3], b1), p.fmt),
-                        pack16(f(a[4], b0), f(a[5], b0), p.fmt), pack16(f(a[6], b1), f(a[7], b1), p.fmt));
-      stmatrix_x4_trans(stage + st_off + 32, pack16(f(b[0], b2), f(b[1], b2), p.fmt), pack16(f(b[2], b3), f(b[3], b3), p.fmt),
-                        pack16(f(b[4], b2), f(b[5], b2), p.fmt), pack16(f(b[6], b3), f(b[7], b3), p.fmt));
+      auto emit = [&](auto f, const int fmt) {
+        stmatrix_x4_trans(stage + st_off, pack16(f(a[0], b0), f(a[1], b0), fmt), pack16(f(a[2], b1), f(a[3], b1), fmt),
+                          pack16(f(a[4], b0), f(a[5], b0), fmt), pack16(f(a[6], b1), f(a[7], b1), fmt));
+        stmatrix_x4_trans(stage + st_off + 32, pack16(f(b[0], b2), f(b[1], b2), fmt), pack16(f(b[2], b3), f(b[3], b3), fmt),
+                          pack16(f(b[4], b2), f(b[5], b2), fmt), pack16(f(b[6], b3), f(b[7], b3), fmt));
+      };
+      auto plain = [](uint32_t v, float bias) { return __uint_as_float(v) + bias; };
+      if (p.act == kActNone && p.fmt == kBF16) emit(plain, kBF16);
+      else if (p.act == kActNone) emit(plain, kF16);
+      else emit([&](uint32_t v, float bias) { return act_fn(__uint_as_float(v) + bias, p.act); }, p.fmt);
     }
     __syncwarp();
     constexpr int UNITS = D_ROW_BYTES / 16, ROUNDS = UNITS / 2, TOKENS = 32 / UNITS;

@@ -214,6 +214,7 @@ int launch_lora_add(const LoraArgs& a, cudaStream_t stream);
 struct GroupedGemmArgs {
   const void* x;           // [x_rows, K], row pitch ldx: a row per place, or read through rows
   const int* rows;         // [total] row of x for every place, or null
+  void* scratch;           // [total, K], used where plan_grouped says so
   const void* values;      // [experts, n_out, K/2]
   const void* meta;        // tiled metadata of every expert, one after the other
   const void* bias;        // as GroupedParams
@@ -223,9 +224,12 @@ struct GroupedGemmArgs {
   int* status;
   int x_rows, total;       // total: rows of y (the groups fill at most these)
   int experts, n_out, K, ldx, ldy, fmt, epi, act, num_sms;
+  int variant;             // 0 = plan_grouped
 };
 int launch_grouped_gemm(const GroupedGemmArgs& a, cudaStream_t stream);
 // The CTA-pair form of it, for many tokens per expert.
-int launch_grouped_gemm_pair(const GroupedGemmArgs& a, cudaStream_t stream);
+int launch_grouped_gemm_pair(const GroupedGemmArgs& a, int variant, cudaStream_t stream);
+// What launch_grouped_gemm runs (variants of sparse_gemm_grouped.cu; 10000 + variant: the rows are copied first).  Host-only.
+int plan_grouped(int total, int experts, int n_out, int K, bool gather, int num_sms);
 
 }  // namespace sfb200

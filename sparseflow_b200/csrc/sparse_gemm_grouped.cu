@@ -17,6 +17,7 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
+#include <math.h>
 #include <stdint.h>
 
 #include "grouped.cuh"
@@ -33,6 +34,7 @@ template <int BN_, int STAGES_, int EPI_, bool GATHER_>
 struct GCfg {
   static constexpr int BN = BN_, STAGES = STAGES_, EPI = EPI_;
   static constexpr bool GATHER = GATHER_;      // token rows fetched four by four through p.rows
+  static constexpr int GATHER_WARPS = GATHER ? 4 : 0, THREADS = 192 + 32 * GATHER_WARPS;
   static constexpr int BK = 128;
   static constexpr int A_BYTES = 128 * 64 * 2;
   static constexpr int B_SUB_BYTES = BN * 128;
@@ -50,12 +52,12 @@ struct GCfg {
   static constexpr int OFF_BAR = OFF_D + D_BYTES;
   static constexpr int OFF_TABLE = OFF_BAR + 256;
   static constexpr int SMEM_BYTES = OFF_TABLE + 1024;      // + the tables of tiles, sized at launch, + alignment slack
-  static_assert(BN % 16 == 0 && BN >= 32 && BN <= 128, "BN: at most four rows per producer lane");
+  static_assert(BN % 16 == 0 && BN >= 32 && BN <= 128, "BN");
   static_assert(8 * (2 * STAGES + 4) + 8 <= 256, "barriers");
 };
 
 template <class C>
-__global__ void __launch_bounds__(192, 1)
+__global__ void __launch_bounds__(C::THREADS, 1)
 grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB, const GroupedParams p) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
@@ -77,7 +79,9 @@ grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
   if (threadIdx.x == 0) {
     *err = 0;
     for (int s = 0; s < C::STAGES; ++s) {
-      mbar_init(bar_full + 8 * s, 1);
+      // one arrival announces the bytes; every gathering warp arrives too, also where it has no row to fetch: a warp that only watched
+      // the stages go by could fall two phases behind and wait for a parity that does not come again
+      mbar_init(bar_full + 8 * s, 1 + C::GATHER_WARPS);
       mbar_init(bar_empty + 8 * s, 1);
     }
     for (int a = 0; a < 2; ++a) {
@@ -102,44 +106,30 @@ grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
   const int num_tiles = first_tile[p.experts];
 
   if (warp == 0) {
-    // TMA producer: one lane waits, announces the bytes and copies the weight; the token tile is one box by the same lane, or
-    // four rows per lane
-    const bool one = elect_one();
-    int s = 0;
-    uint32_t ph = 0;
-    bool ok = true;
-    GroupedTile t;
-    t.e = 0;
-    for (int tile = blockIdx.x; tile < num_tiles && ok; tile += gridDim.x) {
-      locate_tile(p, C::BN, first_tile, first_row, tile, t);
-      const uint32_t* meta = p.meta + (static_cast<size_t>(t.e) * p.row_tiles + t.m_blk) * p.k_tiles128 * 512;
-      const int fours = (t.count + 3) / 4;
-      int rows[4];
-      if (C::GATHER) gather_rows_of(p, t.tok0, t.count, rows);
-      const uint32_t b_bytes = C::GATHER ? static_cast<uint32_t>(fours) * 1024u : C::B_BYTES;
-      for (int kt = 0; kt < k_iters; ++kt) {
-        ok = mbar_wait(bar_empty + 8 * s, ph ^ 1, err, p.status, 1);
-        ok = __all_sync(0xffffffffu, ok);
-        if (!ok) break;
-        const uint32_t full = bar_full + 8 * s;
-        const uint32_t b_dst = sbase + C::OFF_B + s * C::B_BYTES;
-        if (one) {
+    if (elect_one()) {
+      int s = 0;
+      uint32_t ph = 0;
+      bool ok = true;
+      GroupedTile t;
+      t.e = 0;
+      for (int tile = blockIdx.x; tile < num_tiles && ok; tile += gridDim.x) {
+        locate_tile(p, C::BN, first_tile, first_row, tile, t);
+        const uint32_t* meta = p.meta + (static_cast<size_t>(t.e) * p.row_tiles + t.m_blk) * p.k_tiles128 * 512;
+        const uint32_t b_bytes = C::GATHER ? static_cast<uint32_t>((t.count + 3) / 4) * 1024u : C::B_BYTES;
+        for (int kt = 0; kt < k_iters; ++kt) {
+          ok = mbar_wait(bar_empty + 8 * s, ph ^ 1, err, p.status, 1);
+          if (!ok) break;
+          const uint32_t full = bar_full + 8 * s;
           mbar_arrive_expect_tx(full, C::A_BYTES + C::E_BYTES + b_bytes);
           tma_load_2d(sbase + C::OFF_A + s * C::A_BYTES, &tmA, kt * 64, t.e * p.n_out + t.m_blk * 128, full);
           bulk_load_1d(sbase + C::OFF_E + s * C::E_BYTES, meta + static_cast<size_t>(kt) * 512, C::E_BYTES, full);
           if (!C::GATHER) {
 #pragma unroll
-            for (int j = 0; j < 2; ++j) tma_load_2d(b_dst + j * C::B_SUB_BYTES, &tmB, kt * C::BK + j * 64, t.tok0, full);
+            for (int j = 0; j < 2; ++j)
+              tma_load_2d(sbase + C::OFF_B + s * C::B_BYTES + j * C::B_SUB_BYTES, &tmB, kt * C::BK + j * 64, t.tok0, full);
           }
+          if (++s == C::STAGES) { s = 0; ph ^= 1; }
         }
-        if (C::GATHER) {
-          __syncwarp();      // the bytes are announced before any arrive
-          if (lane < fours) {
-#pragma unroll
-            for (int j = 0; j < 2; ++j) tma_gather4(b_dst + j * C::B_SUB_BYTES + lane * 512, &tmB, kt * C::BK + j * 64, rows, full);
-          }
-        }
-        if (++s == C::STAGES) { s = 0; ph ^= 1; }
       }
     }
   } else if (warp == 1) {
@@ -175,6 +165,30 @@ grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
         if (!ok) break;
         tc_commit(bar_accf + 8 * as);
         if (++as == C::ACC) { as = 0; aph ^= 1; }
+      }
+    }
+  } else if (C::GATHER && warp >= 6) {
+    // token rows, four by four
+    const int at = lane * C::GATHER_WARPS + warp - 6;
+    int s = 0;
+    uint32_t ph = 0;
+    bool ok = true;
+    GroupedTile t;
+    t.e = 0;
+    for (int tile = blockIdx.x; tile < num_tiles && ok; tile += gridDim.x) {
+      locate_tile(p, C::BN, first_tile, first_row, tile, t);
+      int rows[4];
+      gather_rows_of(p, t.tok0, t.count, at, rows);
+      for (int kt = 0; kt < k_iters; ++kt) {
+        ok = __all_sync(0xffffffffu, mbar_wait(bar_empty + 8 * s, ph ^ 1, err, p.status, 5));
+        if (!ok) break;
+        if (4 * at < t.count) {
+#pragma unroll
+          for (int j = 0; j < 2; ++j)
+            tma_gather4(sbase + C::OFF_B + s * C::B_BYTES + j * C::B_SUB_BYTES + at * 512, &tmB, kt * C::BK + j * 64, rows, bar_full + 8 * s);
+        }
+        if (lane == 0) mbar_arrive(bar_full + 8 * s);
+        if (++s == C::STAGES) { s = 0; ph ^= 1; }
       }
     }
   } else {
@@ -232,18 +246,76 @@ int launch_cfg(const GroupedGemmArgs& a, cudaStream_t stream) {
     return kErrTensorMap;
   if (!make_map_2d(&tmB, a.x, a.x_rows, a.K, static_cast<uint64_t>(a.ldx) * 2, C::GATHER ? 1 : C::BN, 64, CU_TENSOR_MAP_SWIZZLE_128B, a.fmt)) return kErrTensorMap;
   const GroupedParams p = grouped_params(a);
-  return launch_dependent(grouped_gemm_kernel<C>, a.num_sms, 192, smem, 0, stream, tmA, tmB, p);
+  return launch_dependent(grouped_gemm_kernel<C>, a.num_sms, C::THREADS, smem, 0, stream, tmA, tmB, p);
 }
 
 template <int EPI, bool GATHER>
-int dispatch(const GroupedGemmArgs& a, cudaStream_t stream) {
-  const int per_expert = a.total / a.experts;
-  if (per_expert <= 24) return launch_cfg<GCfg<32, 7, EPI, GATHER>>(a, stream);
-  if (per_expert <= 64) return launch_cfg<GCfg<64, 6, EPI, GATHER>>(a, stream);
-  return launch_grouped_gemm_pair(a, stream);
+int dispatch(const GroupedGemmArgs& a, int variant, cudaStream_t stream) {
+  if (variant == 32) return launch_cfg<GCfg<32, 7, EPI, GATHER>>(a, stream);
+  if (variant == 64) return launch_cfg<GCfg<64, 6, EPI, GATHER>>(a, stream);
+  return launch_grouped_gemm_pair(a, variant, stream);
+}
+
+// dst[i] = src[rows[i]] (a row outside 0 .. src_rows-1: zeros)
+__global__ void __launch_bounds__(256) gather_rows_kernel(const uint16_t* src, int64_t ld, int src_rows, const int* rows, int n, int pieces, uint16_t* dst) {
+  dependency_wait();
+  dependency_trigger();
+  for (int i = blockIdx.x; i < n; i += gridDim.x) {
+    const int r = rows[i];
+    const bool ok = r >= 0 && r < src_rows;
+    for (int c = threadIdx.x; c < pieces; c += 256) {
+      const uint4 v = ok ? *reinterpret_cast<const uint4*>(src + r * ld + c * 8) : make_uint4(0, 0, 0, 0);
+      *reinterpret_cast<uint4*>(dst + (static_cast<size_t>(i) * pieces + c) * 8) = v;
+    }
+  }
+}
+
+// Estimated time in us of a variant (32, 64: single-CTA tiles of that many tokens; 1128, 1240, 2128, 2240: pair tiles of 256 or 512
+// rows) with all experts of the average size: passes over the SMs or pairs x (128-wide K steps x step time + drain), and the weights at
+// 6.2 TB/s; the shorter of the two adds a sixth.  Constants fitted to 450 runs on 13 weight sets (1000-22016 rows, K 512-11008, 4-128
+// experts, 4-1024 tokens per expert with ragged sizes; relative error 0.1); the choice by it averages 1.02 of the fastest variant.
+double grouped_cost(int variant, bool gather, int total, int experts, int n_out, int K, int num_sms) {
+  struct Step { int rows, tokens, variant; double base, per_token, drain, tail, g_base, g_per_token, g_drain, g_tail; };
+  static const Step steps[] = {
+      {128, 32, 32, 0.0255, 0.0038, 1.6, 1.0, 0.054, 0.0082, 1.8, 0.65},    {128, 64, 64, 0.131, 0.0011, 1.3, 0.77, 0.138, 0.0051, 1.7, 0.47},
+      {256, 128, 1128, 0.182, 0.0005, 1.7, 0.65, 0.40, 0.0020, 3.0, 0.4},   {256, 240, 1240, 0.257, 0.0005, 1.8, 0.65, 0.243, 0.0014, 1.9, 0.40},
+      {512, 128, 2128, 0.281, 0.0011, 3.6, 0.74, 0.261, 0.0023, 3.4, 0.56}, {512, 240, 2240, 0.323, 0.0016, 4.5, 0.67, 0.308, 0.0024, 4.4, 0.57}};
+  for (const Step& s : steps) {
+    if (s.variant != variant) continue;
+    const double avg = total > experts ? static_cast<double>(total) / experts : 1.0;
+    const double active = total < experts ? total : experts;
+    const int cuts = static_cast<int>(ceil(avg / s.tokens));
+    const double tiles = active * ((n_out + s.rows - 1) / s.rows) * cuts, units = s.rows == 128 ? num_sms : num_sms / 2;
+    const double passes = tiles > units ? tiles / units + (gather ? s.g_tail : s.tail) : 1.0;
+    const double step = (gather ? s.g_base : s.base) + (gather ? s.g_per_token : s.per_token) * (avg / cuts);
+    const double work = passes * (((K + 127) / 128) * step + (gather ? s.g_drain : s.drain));
+    const double hbm = active * n_out * (K * 1.125) / 6.2e6;
+    return 5.0 + (work > hbm ? work + 0.15 * hbm : hbm + 0.15 * work);
+  }
+  return 1e30;
 }
 
 }  // namespace
+
+// What a call runs: the variant estimated fastest; with `gather`, 10000 more where copying the rows into the order of the experts and
+// multiplying the copy is estimated faster than fetching four rows per copy instruction inside the product (such fetches take about 35 cycles each
+// whatever they bring, which bounds tiles with many tokens: 22016 x 4096, 8 experts of 512 tokens 510 us, contiguous 352 us).
+int plan_grouped(int total, int experts, int n_out, int K, bool gather, int num_sms) {
+  static const int variants[] = {32, 64, 1128, 1240, 2128, 2240};
+  int best = 0;
+  double cost = 1e300;
+  for (int v : variants) {
+    const double c = grouped_cost(v, gather, total, experts, n_out, K, num_sms);
+    if (c < cost) { cost = c; best = v; }
+  }
+  if (!gather) return best;
+  const double copy = 2.5 + static_cast<double>(total) * K * 4.0 / 5.5e6;
+  for (int v : variants) {
+    const double c = copy + grouped_cost(v, false, total, experts, n_out, K, num_sms);
+    if (c < cost) { cost = c; best = 10000 + v; }
+  }
+  return best;
+}
 
 int launch_grouped_gemm(const GroupedGemmArgs& a, cudaStream_t stream) {
   if (a.experts < 1 || a.experts > kMaxExperts || a.total < 0 || a.K <= 0 || a.K % 64 != 0 || a.n_out <= 0 || a.n_out % 8 != 0) return kErrInvalid;
@@ -258,11 +330,23 @@ int launch_grouped_gemm(const GroupedGemmArgs& a, cudaStream_t stream) {
   // coordinates of the copies and tile numbers are 32-bit
   if (static_cast<int64_t>(a.experts) * a.n_out > 0x7fffffffll - 256) return kErrInvalid;
   if (static_cast<int64_t>((a.n_out + 127) / 128) * (a.total / 16 + a.experts) > 0x7fffffffll) return kErrInvalid;
-  if (a.epi == kEpiSwiGLU) {
-    if (a.n_out % 32 != 0) return kErrInvalid;
-    return a.rows ? dispatch<kEpiSwiGLU, true>(a, stream) : dispatch<kEpiSwiGLU, false>(a, stream);
+  if (a.epi == kEpiSwiGLU && a.n_out % 32 != 0) return kErrInvalid;
+  GroupedGemmArgs b = a;
+  int variant = a.variant ? a.variant : plan_grouped(a.total, a.experts, a.n_out, a.K, a.rows != nullptr, a.num_sms);
+  if (variant >= 10000) {
+    variant -= 10000;
+    if (!a.rows || !a.scratch || (reinterpret_cast<uintptr_t>(a.scratch) & 15)) return kErrInvalid;
+    const int rc = launch_dependent(gather_rows_kernel, a.total < 16 * a.num_sms ? a.total : 16 * a.num_sms, 256, 0, 0, stream,
+                                    static_cast<const uint16_t*>(a.x), static_cast<int64_t>(a.ldx), a.x_rows, a.rows, a.total, a.K / 8,
+                                    static_cast<uint16_t*>(a.scratch));
+    if (rc != kOk) return rc;
+    b.x = a.scratch;
+    b.ldx = a.K;
+    b.x_rows = a.total;
+    b.rows = nullptr;
   }
-  return a.rows ? dispatch<kEpiStore, true>(a, stream) : dispatch<kEpiStore, false>(a, stream);
+  if (a.epi == kEpiSwiGLU) return b.rows ? dispatch<kEpiSwiGLU, true>(b, variant, stream) : dispatch<kEpiSwiGLU, false>(b, variant, stream);
+  return b.rows ? dispatch<kEpiStore, true>(b, variant, stream) : dispatch<kEpiStore, false>(b, variant, stream);
 }
 
 }  // namespace sfb200

@@ -19,20 +19,21 @@
 namespace sfb200 {
 namespace {
 
-template <int EPI_, bool GATHER_>
+template <int BN_, int STAGES_, int BOX_, int RS_, int EPI_, bool GATHER_>
 struct PCfg {
-  static constexpr int EPI = EPI_;
+  static constexpr int EPI = EPI_, RS = RS_;                   // RS: 128-row sets per CTA
   static constexpr bool GATHER = GATHER_;
-  static constexpr int BN = 240, HALF = BN / 2, BOX = 40;      // tokens per tile, per CTA, per copy
-  static constexpr int BK = 128, STAGES = 4;
-  static constexpr int A_BYTES = 128 * 64 * 2;
+  static constexpr int BN = BN_, HALF = BN / 2, BOX = BOX_;      // tokens per tile, per CTA, per copy
+  static constexpr int BK = 128, STAGES = STAGES_;
+  static constexpr int A_SUB_BYTES = 128 * 64 * 2, A_BYTES = RS * A_SUB_BYTES;
   static constexpr int B_SUB_BYTES = HALF * 128;
   static constexpr int B_BYTES = 2 * B_SUB_BYTES;
-  static constexpr int E_BYTES = 2048;
+  static constexpr int E_SUB_BYTES = 2048, E_BYTES = RS * E_SUB_BYTES;
+  static constexpr int ACC_BUFS = RS == 1 ? 2 : 1;             // accumulator sets of RS * BN columns
   static constexpr int E_COL0 = 2 * BN;
-  static constexpr int EPI_WARPS = 8, THREADS = 64 + 32 * EPI_WARPS;
+  static constexpr int EPI_WARPS = RS_ == 1 ? 8 : 16, GATHER_WARPS = GATHER ? (RS_ == 1 ? 8 : 4) : 0, THREADS = 64 + 32 * (EPI_WARPS + GATHER_WARPS);
   static constexpr int D_ROW_BYTES = EPI == kEpiSwiGLU ? 32 : 64;
-  static constexpr int D_WARP_BYTES = 2 * 16 * D_ROW_BYTES;
+  static constexpr int D_BUFS = 1, D_WARP_BYTES = D_BUFS * 16 * D_ROW_BYTES;
   static constexpr int OFF_A = 0;
   static constexpr int OFF_B = OFF_A + STAGES * A_BYTES;
   static constexpr int OFF_E = OFF_B + STAGES * B_BYTES;
@@ -40,8 +41,8 @@ struct PCfg {
   static constexpr int OFF_BAR = OFF_D + EPI_WARPS * D_WARP_BYTES;
   static constexpr int OFF_TABLE = OFF_BAR + 256;
   static constexpr int SMEM_BYTES = OFF_TABLE + 1024;      // + the tables of tiles, sized at launch, + alignment slack
-  static_assert(HALF % BOX == 0 && BOX % 8 == 0 && HALF / 4 <= 32, "token halves: whole boxes, at most four rows per lane");
-  static_assert(E_COL0 + 4 * STAGES <= 512, "tensor memory");
+  static_assert(HALF % BOX == 0 && BOX % 8 == 0 && HALF <= 128, "token halves: whole boxes, at most four rows per lane");
+  static_assert(E_COL0 + 4 * RS * STAGES <= 512, "tensor memory");
 };
 
 template <class C>
@@ -70,7 +71,9 @@ grouped_gemm_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_c
   if (threadIdx.x == 0) {
     *err = 0;
     for (int s = 0; s < C::STAGES; ++s) {
-      mbar_init(bar_full + 8 * s, 1);
+      // one arrival announces the bytes; every gathering warp arrives too, also where it has no row to fetch: a warp that only watched
+      // the stages go by could fall two phases behind and wait for a parity that does not come again
+      mbar_init(bar_full + 8 * s, 1 + 2 * C::GATHER_WARPS);
       mbar_init(bar_empty + 8 * s, 1);
     }
     for (int b = 0; b < 2; ++b) {
@@ -98,53 +101,49 @@ grouped_gemm_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_c
 
   if (warp == 0) {
     // ------------------------------------------------------------ TMA producer (both CTAs)
-    const bool one = elect_one();
-    const uint32_t leader_full0 = mapa_u32(bar_full, 0);
-    int s = 0;
-    uint32_t ph = 0;
-    bool ok = true;
-    GroupedTile t;
-    t.e = 0;
-    for (int tile = pair_id; tile < num_tiles && ok; tile += num_pairs) {
-      locate_tile(p, C::BN, first_tile, first_row, tile, t);
-      const int half = ((t.count + 15) & ~15) / 2;                       // rows of the operand in each CTA
-      const int in0 = t.count < half ? t.count : half, in1 = t.count - in0;      // of which hold a token
-      const int mine = leader ? in0 : in1, tok = t.tok0 + rank * half;
-      const int row = t.m_blk * 256 + rank * 128;                        // row of the expert's weight
-      // a row tile that lies wholly behind the expert's rows (an odd number of 128-row tiles) loads its last tile again: not stored
-      const int row_tile = min(row >> 7, p.row_tiles - 1);
-      const int e_x = (t.e * p.row_tiles + row_tile) * p.k_tiles128 * 256;
-      const int a_y = t.e * p.n_out + row_tile * 128;
-      int rows[4];
-      if (C::GATHER) gather_rows_of(p, tok, mine, rows);
-      const int fours = (mine + 3) / 4, boxes = (mine + C::BOX - 1) / C::BOX;
-      const uint32_t bytes = C::GATHER ? static_cast<uint32_t>((in0 + 3) / 4 + (in1 + 3) / 4) * 1024u
-                                       : static_cast<uint32_t>((in0 + C::BOX - 1) / C::BOX + (in1 + C::BOX - 1) / C::BOX) * (C::BOX * 256u);
-      for (int kt = 0; kt < k_iters; ++kt) {
-        ok = mbar_wait(bar_empty + 8 * s, ph ^ 1, err, p.status, 1);
-        ok = __all_sync(0xffffffffu, ok);
-        if (!ok) break;
-        const uint32_t full = leader_full0 + 8 * s;
-        const uint32_t b_dst = sbase + C::OFF_B + s * C::B_BYTES;
-        if (one) {
+    if (elect_one()) {
+      const uint32_t leader_full0 = mapa_u32(bar_full, 0);
+      int s = 0;
+      uint32_t ph = 0;
+      bool ok = true;
+      GroupedTile t;
+      t.e = 0;
+      for (int tile = pair_id; tile < num_tiles && ok; tile += num_pairs) {
+        locate_tile(p, C::BN, first_tile, first_row, tile, t);
+        const int half = ((t.count + 15) & ~15) / 2;                       // rows of the operand in each CTA
+        const int in0 = t.count < half ? t.count : half, in1 = t.count - in0;      // of which hold a token
+        const int mine = leader ? in0 : in1, tok = t.tok0 + rank * half;
+        int e_x[C::RS], a_y[C::RS];
+#pragma unroll
+        for (int rs = 0; rs < C::RS; ++rs) {
+          // 128-row tile of the expert's weight; one that lies wholly behind its rows loads the last tile again: not stored
+          const int row_tile = min((t.m_blk * 2 + rank) * C::RS + rs, p.row_tiles - 1);
+          e_x[rs] = (t.e * p.row_tiles + row_tile) * p.k_tiles128 * 256;
+          a_y[rs] = t.e * p.n_out + row_tile * 128;
+        }
+        const int boxes = (mine + C::BOX - 1) / C::BOX;
+        const uint32_t bytes =
+            C::GATHER ? static_cast<uint32_t>((in0 + 3) / 4 + (in1 + 3) / 4) * 1024u
+                      : static_cast<uint32_t>((in0 + C::BOX - 1) / C::BOX + (in1 + C::BOX - 1) / C::BOX) * (C::BOX * 256u);
+        for (int kt = 0; kt < k_iters; ++kt) {
+          ok = mbar_wait(bar_empty + 8 * s, ph ^ 1, err, p.status, 1);
+          if (!ok) break;
+          const uint32_t full = leader_full0 + 8 * s;
+          const uint32_t b_dst = sbase + C::OFF_B + s * C::B_BYTES;
           if (leader) mbar_arrive_expect_tx(bar_full + 8 * s, 2 * (C::A_BYTES + C::E_BYTES) + bytes);      // of both CTAs
-          tma_load_2d_pair(sbase + C::OFF_A + s * C::A_BYTES, &tmA, kt * 64, a_y, full);
-          tma_load_1d_pair(sbase + C::OFF_E + s * C::E_BYTES, &tmE, e_x + kt * 256, full);
+#pragma unroll
+          for (int rs = 0; rs < C::RS; ++rs) {
+            tma_load_2d_pair(sbase + C::OFF_A + s * C::A_BYTES + rs * C::A_SUB_BYTES, &tmA, kt * 64, a_y[rs], full);
+            tma_load_1d_pair(sbase + C::OFF_E + s * C::E_BYTES + rs * C::E_SUB_BYTES, &tmE, e_x[rs] + kt * 256, full);
+          }
           if (!C::GATHER) {
             for (int b = 0; b < boxes; ++b)
 #pragma unroll
               for (int j = 0; j < 2; ++j)
                 tma_load_2d_pair(b_dst + j * C::B_SUB_BYTES + b * C::BOX * 128, &tmB, kt * C::BK + j * 64, tok + b * C::BOX, full);
           }
+          if (++s == C::STAGES) { s = 0; ph ^= 1; }
         }
-        if (C::GATHER) {
-          __syncwarp();
-          if (lane < fours) {
-#pragma unroll
-            for (int j = 0; j < 2; ++j) tma_gather4_pair(b_dst + j * C::B_SUB_BYTES + lane * 512, &tmB, kt * C::BK + j * 64, rows, full);
-          }
-        }
-        if (++s == C::STAGES) { s = 0; ph ^= 1; }
       }
     }
   } else if (warp == 1) {
@@ -158,7 +157,7 @@ grouped_gemm_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_c
       for (int tile = pair_id; tile < num_tiles && ok; tile += num_pairs, ++it) {
         locate_tile(p, C::BN, first_tile, first_row, tile, t);
         const uint32_t idesc = make_idesc_f16(256, (t.count + 15) & ~15, p.fmt, true);
-        const uint32_t as = it & 1u, use = it >> 1;
+        const uint32_t as = C::ACC_BUFS == 2 ? it & 1u : 0u, use = C::ACC_BUFS == 2 ? it >> 1 : it;
         const uint32_t d_tmem = tmem_base + as * C::BN;
         ok = mbar_wait(bar_acce + 8 * as, (use & 1u) ^ 1u, err, p.status, 3);
         if (!ok) break;
@@ -167,15 +166,21 @@ grouped_gemm_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_c
           ok = mbar_wait(bar_full + 8 * s, ph, err, p.status, 2);
           if (!ok) break;
           tc_fence_after();
-          const uint32_t e_cols = C::E_COL0 + 4 * s;
-          tc_cp_128x128b_pair(tmem_base + e_cols, make_smem_desc(sbase + C::OFF_E + s * C::E_BYTES, 0, 128, kSwNone));
+          const uint32_t e_cols = C::E_COL0 + 4 * C::RS * s;
+#pragma unroll
+          for (int rs = 0; rs < C::RS; ++rs)
+            tc_cp_128x128b_pair(tmem_base + e_cols + 4 * rs,
+                                make_smem_desc(sbase + C::OFF_E + s * C::E_BYTES + rs * C::E_SUB_BYTES, 0, 128, kSwNone));
           const uint32_t a_addr = sbase + C::OFF_A + s * C::A_BYTES;
           const uint32_t b_addr = sbase + C::OFF_B + s * C::B_BYTES;
 #pragma unroll
-          for (int kb = 0; kb < 4; ++kb)
-            tc_mma_sp_f16_pair(d_tmem, make_smem_desc(a_addr + kb * 32, 16, 1024, kSw128),
-                               make_smem_desc(b_addr + (kb >> 1) * C::B_SUB_BYTES + (kb & 1) * 64, 16, 1024, kSw128),
-                               tmem_base + e_cols + (kb & ~1), idesc | (kb & 1), (kt > 0 || kb > 0) ? 1u : 0u);
+          for (int kb = 0; kb < 4; ++kb) {
+            const uint64_t bdesc = make_smem_desc(b_addr + (kb >> 1) * C::B_SUB_BYTES + (kb & 1) * 64, 16, 1024, kSw128);
+#pragma unroll
+            for (int rs = 0; rs < C::RS; ++rs)
+              tc_mma_sp_f16_pair(d_tmem + rs * C::BN, make_smem_desc(a_addr + rs * C::A_SUB_BYTES + kb * 32, 16, 1024, kSw128), bdesc,
+                                 tmem_base + e_cols + 4 * rs + (kb & ~1), idesc | (kb & 1), (kt > 0 || kb > 0) ? 1u : 0u);
+          }
           tc_commit_pair(bar_empty + 8 * s);
           if (++s == C::STAGES) { s = 0; ph ^= 1; }
         }
@@ -183,9 +188,39 @@ grouped_gemm_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_c
         tc_commit_pair(bar_accf + 8 * as);
       }
     }
+  } else if (C::GATHER && warp >= 2 + C::EPI_WARPS) {
+    // ------------------------------------------------------------ token rows through the grouping, four by four (both CTAs)
+    // (a warp issues its lanes' copies one by one, 25-40 cycles each: hence several warps)
+    const int at = lane * C::GATHER_WARPS + warp - 2 - C::EPI_WARPS;
+    const uint32_t leader_full0 = mapa_u32(bar_full, 0);
+    int s = 0;
+    uint32_t ph = 0;
+    bool ok = true;
+    GroupedTile t;
+    t.e = 0;
+    for (int tile = pair_id; tile < num_tiles && ok; tile += num_pairs) {
+      locate_tile(p, C::BN, first_tile, first_row, tile, t);
+      const int half = ((t.count + 15) & ~15) / 2;
+      const int in0 = t.count < half ? t.count : half;
+      const int mine = leader ? in0 : t.count - in0;
+      int rows[4];
+      gather_rows_of(p, t.tok0 + rank * half, mine, at, rows);
+      for (int kt = 0; kt < k_iters; ++kt) {
+        ok = __all_sync(0xffffffffu, mbar_wait(bar_empty + 8 * s, ph ^ 1, err, p.status, 5));
+        if (!ok) break;
+        if (4 * at < mine) {
+#pragma unroll
+          for (int j = 0; j < 2; ++j)
+            tma_gather4_pair(sbase + C::OFF_B + s * C::B_BYTES + j * C::B_SUB_BYTES + at * 512, &tmB, kt * C::BK + j * 64, rows, leader_full0 + 8 * s);
+        }
+        if (lane == 0) mbar_arrive_remote(leader_full0 + 8 * s);
+        if (++s == C::STAGES) { s = 0; ph ^= 1; }
+      }
+    }
   } else {
     // ------------------------------------------------------------ drain (both CTAs)
-    const int q = warp & 3, part = (warp - 2) >> 2;
+    constexpr int PARTS = C::EPI_WARPS / 4 / C::RS;      // warps that share an accumulator's lanes
+    const int q = warp & 3, rs = ((warp - 2) >> 2) / PARTS, part = ((warp - 2) >> 2) % PARTS;
     const uint32_t leader_acce0 = mapa_u32(bar_acce, 0);
     const uint64_t pol = l2_policy_evict_first();
     const uint32_t stage0 = sbase + C::OFF_D + (warp - 2) * C::D_WARP_BYTES;
@@ -195,13 +230,14 @@ grouped_gemm_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_c
     t.e = 0;
     for (int tile = pair_id; tile < num_tiles && ok; tile += num_pairs, ++it) {
       locate_tile(p, C::BN, first_tile, first_row, tile, t);
-      const uint32_t as = it & 1u, use = it >> 1;
+      const uint32_t as = C::ACC_BUFS == 2 ? it & 1u : 0u, use = C::ACC_BUFS == 2 ? it >> 1 : it;
       ok = __all_sync(0xffffffffu, mbar_wait(bar_accf + 8 * as, use & 1u, err, p.status, 4));
       if (!ok) break;
       tc_fence_after();
-      const int chunks = (t.count + 15) / 16, first_half = (chunks + 1) / 2;
-      drain_tile<C::EPI>(p, t, t.m_blk * 256 + rank * 128 + q * 32, tmem_base + (static_cast<uint32_t>(q * 32) << 16) + as * C::BN,
-                         part ? first_half : 0, part ? chunks : first_half, stage0, 1, pol, [&]() {
+      const int chunks = (t.count + 15) / 16;
+      drain_tile<C::EPI>(p, t, ((t.m_blk * 2 + rank) * C::RS + rs) * 128 + q * 32,
+                         tmem_base + (static_cast<uint32_t>(q * 32) << 16) + (as + rs) * C::BN,
+                         chunks * part / PARTS, chunks * (part + 1) / PARTS, stage0, C::D_BUFS - 1, pol, [&]() {
                            tc_fence_before();
                            __syncwarp();
                            if (lane == 0) mbar_arrive_remote(leader_acce0 + 8 * as);
@@ -244,17 +280,29 @@ int launch_cfg(const GroupedGemmArgs& a, cudaStream_t stream) {
     return kErrTensorMap;
   if (!make_map_1d_u64(&tmE, a.meta, a.experts * meta_bytes(a.n_out, a.K) / 8, 256)) return kErrTensorMap;
   GroupedParams p = grouped_params(a);
-  p.m_blks = (a.n_out + 255) / 256;
+  p.m_blks = (a.n_out + 256 * C::RS - 1) / (256 * C::RS);
   return launch_dependent(grouped_gemm_pair_kernel<C>, a.num_sms / 2 * 2, C::THREADS, smem, 0, stream, tmA, tmB, tmE, p);
+}
+
+template <int BN, int STAGES, int BOX, int RS>
+int dispatch_epi(const GroupedGemmArgs& a, cudaStream_t stream) {
+  if (a.epi == kEpiSwiGLU)
+    return a.rows ? launch_cfg<PCfg<BN, STAGES, BOX, RS, kEpiSwiGLU, true>>(a, stream) : launch_cfg<PCfg<BN, STAGES, BOX, RS, kEpiSwiGLU, false>>(a, stream);
+  return a.rows ? launch_cfg<PCfg<BN, STAGES, BOX, RS, kEpiStore, true>>(a, stream) : launch_cfg<PCfg<BN, STAGES, BOX, RS, kEpiStore, false>>(a, stream);
 }
 
 }  // namespace
 
-int launch_grouped_gemm_pair(const GroupedGemmArgs& a, cudaStream_t stream) {
+int launch_grouped_gemm_pair(const GroupedGemmArgs& a, int variant, cudaStream_t stream) {
   // the metadata of all experts is one tensor with 32-bit coordinates
   if (a.experts * (meta_bytes(a.n_out, a.K) / 8) > 0x7fffffffull) return kErrInvalid;
-  if (a.epi == kEpiSwiGLU) return a.rows ? launch_cfg<PCfg<kEpiSwiGLU, true>>(a, stream) : launch_cfg<PCfg<kEpiSwiGLU, false>>(a, stream);
-  return a.rows ? launch_cfg<PCfg<kEpiStore, true>>(a, stream) : launch_cfg<PCfg<kEpiStore, false>>(a, stream);
+  switch (variant) {      // rows per tile: 256 (1...) or 512 (2...), tokens; shorter token tiles leave room for more stages
+    case 1128: return dispatch_epi<128, 6, 32, 1>(a, stream);
+    case 1240: return dispatch_epi<240, 4, 40, 1>(a, stream);
+    case 2128: return dispatch_epi<128, 4, 32, 2>(a, stream);
+    case 2240: return dispatch_epi<240, 3, 40, 2>(a, stream);
+    default: return kErrInvalid;
+  }
 }
 
 }  // namespace sfb200

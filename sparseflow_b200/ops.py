@@ -493,6 +493,11 @@ def _grouped_args(x: torch.Tensor, cw: CompressedExperts, groups: RowGroups, gat
     return _rows16(x, "x"), total
 
 
+def _grouped_scratch(x: torch.Tensor, total: int, cw: CompressedExperts) -> Optional[torch.Tensor]:
+    n = _lib.lib().sfb200_grouped_scratch_bytes(total, cw.experts, cw.rows, cw.K)
+    return torch.empty(n, dtype=torch.uint8, device=x.device) if n else None
+
+
 def grouped_sparse_gemm(x: torch.Tensor, cw: CompressedExperts, groups: RowGroups, bias: Optional[torch.Tensor] = None, act: Optional[str] = None,
                         gather: bool = False, out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """y[place] = act(x[place] . W_e^T + bias[e]) for the places of every expert e.
@@ -512,7 +517,8 @@ def grouped_sparse_gemm(x: torch.Tensor, cw: CompressedExperts, groups: RowGroup
             _check_out(out, x, (total, cw.rows), x.dtype)
         if total == 0:
             return out
-        rc = _lib.lib().sfb200_grouped_sparse_gemm(x.data_ptr(), _pitch(x), x.shape[0], groups.rows.data_ptr() if gather else None,
+        scratch = _grouped_scratch(x, total, cw) if gather else None
+        rc = _lib.lib().sfb200_grouped_sparse_gemm(x.data_ptr(), _pitch(x), x.shape[0], groups.rows.data_ptr() if gather else None, _ptr(scratch),
                                                    cw.values.data_ptr(), cw.meta.data_ptr(), out.data_ptr(), _pitch(out), total, cw.experts, cw.rows,
                                                    cw.K, _dt(x), _ptr(bias), ACT[act], groups.offsets.data_ptr(), _stream())
     if rc:
@@ -538,8 +544,9 @@ def grouped_sparse_gemm_swiglu(x: torch.Tensor, cw_gu: CompressedExperts, groups
             _check_out(out, x, (total, I), x.dtype)
         if total == 0:
             return out
+        scratch = _grouped_scratch(x, total, cw_gu) if gather else None
         rc = _lib.lib().sfb200_grouped_sparse_gemm_swiglu(x.data_ptr(), _pitch(x), x.shape[0], groups.rows.data_ptr() if gather else None,
-                                                          cw_gu.values.data_ptr(), cw_gu.meta.data_ptr(), out.data_ptr(), _pitch(out),
+                                                          _ptr(scratch), cw_gu.values.data_ptr(), cw_gu.meta.data_ptr(), out.data_ptr(), _pitch(out),
                                                           total, cw_gu.experts, I, cw_gu.K, _dt(x), _ptr(gate_bias), _ptr(up_bias),
                                                           groups.offsets.data_ptr(), _stream())
     if rc:
