@@ -118,18 +118,19 @@ int sfb200_block_norm(const void* x, int64_t ld_x, const void* y, int64_t ld_y, 
   return launch_block_norm(a, static_cast<cudaStream_t>(stream));
 }
 
-size_t sfb200_lora_workspace_bytes(int n, int rank) { return n > 0 && rank > 0 ? static_cast<size_t>(n) * rank * sizeof(float) : 0; }
+size_t sfb200_lora_workspace_bytes(int n, int rank) { return n > 0 && rank > 0 ? lora_workspace_bytes(n, rank) : 0; }
 
 int sfb200_lora_add(const void* y, int64_t ld_y, const void* x, int64_t ld_x, const void* a, const void* b, const float* scales, void* out,
                     int64_t ld_out, int n, int groups, int rank, int K, int N, int dtype, const int* offsets, const int* rows, const int* slots,
                     void* workspace, void* stream) {
   int err = kOk;
-  if (!device_state(&err)) return err;
+  DeviceState* s = device_state(&err);
+  if (!s) return err;
   LoraArgs l{};
   l.y = y; l.x = x; l.a = a; l.b = b; l.scales = scales; l.out = out;
   l.offsets = offsets; l.rows = rows; l.slots = slots; l.workspace = workspace;
   l.ld_y = ld_y; l.ld_x = ld_x; l.ld_out = ld_out;
-  l.n = n; l.groups = groups; l.rank = rank; l.K = K; l.N = N; l.fmt = dtype;
+  l.n = n; l.groups = groups; l.rank = rank; l.K = K; l.N = N; l.fmt = dtype; l.num_sms = s->num_sms;
   return launch_lora_add(l, static_cast<cudaStream_t>(stream));
 }
 

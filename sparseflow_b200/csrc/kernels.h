@@ -199,7 +199,7 @@ struct NormArgs {
 };
 constexpr int kNormMaxCols = 16384;
 int launch_block_norm(const NormArgs& a, cudaStream_t stream);
-// out = y + scales[g] * (x . A_g^T) . B_g^T by the rows' groups.  workspace: n * rank floats.
+// out = y + scales[g] * (x . A_g^T) . B_g^T by the rows' groups.  workspace: lora_workspace_bytes.
 struct LoraArgs {
   const void *y, *x, *a, *b;      // [n, N], [n, K], [groups, rank, K], [groups, N, rank]
   const float* scales;
@@ -207,9 +207,10 @@ struct LoraArgs {
   const int *offsets, *rows, *slots;
   void* workspace;
   int64_t ld_y, ld_x, ld_out;
-  int n, groups, rank, K, N, fmt;
+  int n, groups, rank, K, N, fmt, num_sms;
 };
 int launch_lora_add(const LoraArgs& a, cudaStream_t stream);
+size_t lora_workspace_bytes(int n, int rank);
 // Sparse GEMM grouped by expert: rows offsets[e] .. offsets[e+1] of y through weight e.
 struct GroupedGemmArgs {
   const void* x;           // [x_rows, K], row pitch ldx: a row per place, or read through rows

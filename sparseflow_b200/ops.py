@@ -736,8 +736,9 @@ def lora_add(y: torch.Tensor, x: torch.Tensor, bank: LoraBank, groups: RowGroups
             y = _rows16(y, "y")
             if out.data_ptr() % 16 or _pitch(out) % 8:
                 out = y.new_empty((n, bank.N))
-        work = torch.empty((n, bank.rank), dtype=torch.float32, device=y.device)
-        rc = _lib.lib().sfb200_lora_add(y.data_ptr(), _pitch(y), x.data_ptr(), _pitch(x), bank.a.data_ptr(), bank.b.data_ptr(), bank.scales.data_ptr(),
+        L = _lib.lib()
+        work = torch.empty(L.sfb200_lora_workspace_bytes(n, bank.rank), dtype=torch.uint8, device=y.device)
+        rc = L.sfb200_lora_add(y.data_ptr(), _pitch(y), x.data_ptr(), _pitch(x), bank.a.data_ptr(), bank.b.data_ptr(), bank.scales.data_ptr(),
                                         out.data_ptr(), _pitch(out), n, bank.adapters, bank.rank, bank.K, bank.N, _dt(y), groups.offsets.data_ptr(),
                                         groups.rows.data_ptr(), groups.slots.data_ptr(), work.data_ptr(), _stream())
         if rc:
