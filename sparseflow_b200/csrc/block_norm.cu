@@ -4,13 +4,20 @@
 //   h = norm(r) * weight (+ bias)
 //   norm(v) = v / sqrt(mean(v^2) + eps)                       (rms)
 //           = (v - mean(v)) / sqrt(mean((v - mean(v))^2) + eps)   (layer)
-// h is the norm of the unrounded r.  HBM-bound: x and y are read once, r and h written once; a block owns a row and keeps it in
-// registers between the reductions (one for an rms norm, two for a layer norm, each: the mean first, then the centered
-// squares, so that a large mean costs no digits).
+// h is the norm of the unrounded r.  HBM-bound: x and y are read once, r and h written once.  A block owns a row and keeps it in registers between the
+// reductions: one for an rms norm, two for a layer norm (the mean first, then the centered squares, so that a large mean costs no
+// digits).  x and y wait there in their own type, so that three blocks of a wide row fit an SM and one's loads run under another's reductions.
+//
+// Eight values per access: 16-byte pieces of the tensors, also where a row begins inside one (odd widths): a thread owns
+// the columns of a whole piece, 8j - m .. with m the row's offset, reads it with the neighbour's values in it (inside the tensor) and drops those; the
+// pieces at the ends of a row are stored value by value, and weights, which begin at column 0, are shifted by m from two pieces.
+// Value by value throughout where the tensors' rows do not lie alike in their pieces.
+//   4096 x 8192 (f32 stream, bf16, norm on both sides) 83 us (4.8 TB/s), 16384 x 2048 bf16 58 us, 24 x 4096 2.8 us (latency).
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 #include <stdint.h>
+#include <string.h>
 
 #include "kernels.h"
 #include "launch.h"
@@ -64,125 +71,250 @@ __device__ __forceinline__ void store_f(void* base, int64_t at, const float* f) 
   *reinterpret_cast<Pack<T, V>*>(static_cast<T*>(base) + at) = k;
 }
 
-__device__ __forceinline__ float block_sum(float v, float* part) {
+// Sum over the row's threads (WARP: a warp).  `turn` alternates between two sets of parts, so that one barrier does; the parts are added by
+// every thread, in order, four per load: cheaper than a second round of shuffles.
+template <bool WARP>
+__device__ __forceinline__ float row_sum(float v, float (*part)[32], int& turn) {
 #pragma unroll
   for (int d = 16; d > 0; d >>= 1) v += __shfl_xor_sync(0xffffffffu, v, d);
-  const int warps = blockDim.x >> 5, lane = threadIdx.x & 31;
-  if (warps == 1) return v;
-  __syncthreads();                      // the parts of the sum before are read
-  if (lane == 0) part[threadIdx.x >> 5] = v;
+  if (WARP) return v;
+  const int warps = blockDim.x >> 5;
+  float* mine = part[turn];
+  turn ^= 1;
+  if ((threadIdx.x & 31) == 0) mine[threadIdx.x >> 5] = v;
   __syncthreads();
-  v = lane < warps ? part[lane] : 0.f;
-#pragma unroll
-  for (int d = 16; d > 0; d >>= 1) v += __shfl_xor_sync(0xffffffffu, v, d);
+  v = 0.f;
+  for (int w = 0; w < warps; w += 4) {
+    const float4 q = *reinterpret_cast<const float4*>(mine + w);
+    v += q.x + (w + 1 < warps ? q.y : 0.f) + (w + 2 < warps ? q.z : 0.f) + (w + 3 < warps ? q.w : 0.f);
+  }
   return v;
 }
 
-// f[NV][V]: the thread's values of the row (zero behind its end) -> normalised, weighted
-template <class YT, int V, int NV>
-__device__ __forceinline__ void normalise(float (&f)[NV][V], const NormParams& p, const void* weight, const void* bias, float eps, float* part) {
-  float s = 0.f;
-  if (p.layer) {
+// V values of a row from column c (c may lie before the row, c + V behind it): those of the row, zero for the others.  `room`: values of the tensor
+// from there to its end.
+template <class T, int V, bool SHIFT>
+__device__ __forceinline__ Pack<T, V> load_piece(const void* base, int64_t at, int64_t room) {
+  Pack<T, V> k;
+  if (!SHIFT || room >= V) {
+    k = *reinterpret_cast<const Pack<T, V>*>(static_cast<const T*>(base) + at);
+  } else {
 #pragma unroll
-    for (int n = 0; n < NV; ++n)
+    for (int i = 0; i < V; ++i) k.v[i] = i < room ? static_cast<const T*>(base)[at + i] : from_f<T>(0.f);
+  }
+  return k;
+}
+template <class T, int V, bool SHIFT>
+__device__ __forceinline__ void store_piece(void* base, int64_t at, int c, int cols, const float* f) {
+  if (!SHIFT || (c >= 0 && c + V <= cols)) {
+    store_f<T, V>(base, at, f);
+  } else {
 #pragma unroll
-      for (int i = 0; i < V; ++i) s += f[n][i];
-    const float mean = block_sum(s, part) * p.inv_cols;
-    s = 0.f;
+    for (int i = 0; i < V; ++i)
+      if (c + i >= 0 && c + i < cols) static_cast<T*>(base)[at + i] = from_f<T>(f[i]);
+  }
+}
+// V values of a vector over the columns (whole pieces from column 0, if `pieces`) from column c = 8j - m
+template <class T, int V, bool SHIFT>
+__device__ __forceinline__ void load_vector(const void* base, int64_t first, int c, int cols, int m, bool pieces, float* f) {
+  const T* v = static_cast<const T*>(base) + first;
+  if (!SHIFT || (V == 8 && pieces && m == 0 && c + V <= cols)) {
+    load_f<T, V>(v, c, f);
+  } else if (V == 8 && sizeof(T) == 2 && pieces && c >= 0 && c + m + 8 <= cols) {
+    const uint4 a = *reinterpret_cast<const uint4*>(v + c + m - 8), b = *reinterpret_cast<const uint4*>(v + c + m);
+    uint32_t w[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};      // columns c + m - 8 ..: c is 8 - m values on, the same for the whole block
+    const int off = 8 - m;
+    if (off & 4) {
 #pragma unroll
-    for (int n = 0; n < NV; ++n) {
-      const bool in = (n * blockDim.x + threadIdx.x) * V < static_cast<unsigned>(p.cols);
+      for (int i = 0; i < 6; ++i) w[i] = w[i + 2];
+    }
+    if (off & 2) {
+#pragma unroll
+      for (int i = 0; i < 5; ++i) w[i] = w[i + 1];
+    }
+    if (off & 1) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) w[i] = __funnelshift_r(w[i], w[i + 1], 16);
+    }
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      const uint16_t bits = static_cast<uint16_t>(w[i / 2] >> (16 * (i % 2)));
+      T t;
+      memcpy(&t, &bits, sizeof(T) == 2 ? 2 : 0);
+      f[i] = to_f<T>(t);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < V; ++i) f[i] = c + i >= 0 && c + i < cols ? to_f<T>(v[c + i]) : 0.f;
+  }
+}
+
+// XT: type of x and r; YT: type of y, h, weights and gate.  WARP: a warp per row, eight rows per block; otherwise a block per row.
+template <class XT, class YT, int V, int NV, bool SHIFT, bool LAYER, bool WARP, int MAXT, int MINB>
+__global__ void __launch_bounds__(MAXT, MINB) block_norm_kernel(const NormParams p) {
+  __shared__ __align__(16) float part[2][32];
+  dependency_wait();
+  dependency_trigger();
+  const int row_i = WARP ? static_cast<int>(blockIdx.x * 8 + (threadIdx.x >> 5)) : static_cast<int>(blockIdx.x);
+  if (WARP && row_i >= p.rows) return;
+  const int64_t row = row_i;
+  const int m = SHIFT ? static_cast<int>(row * p.ld_x & 7) : 0;
+  const int c0 = static_cast<int>(WARP ? threadIdx.x & 31 : threadIdx.x) * V - m, step = (WARP ? 32 : static_cast<int>(blockDim.x)) * V;
+  auto outside = [&](int c, int i) { return c + i < 0 || c + i >= p.cols; };
+  int turn = 0;
+  Pack<XT, V> xv[NV];
+  Pack<YT, V> yv[NV];
+#pragma unroll
+  for (int n = 0; n < NV; ++n) {
+    const int c = c0 + n * step;
+    if (c < p.cols) {
+      const int64_t behind = p.rows - 1 - row;
+      xv[n] = load_piece<XT, V, SHIFT>(p.x, row * p.ld_x + c, behind * p.ld_x + p.cols - c);
+      if (p.y != nullptr) yv[n] = load_piece<YT, V, SHIFT>(p.y, row * p.ld_y + c, behind * p.ld_y + p.cols - c);
+    } else {
 #pragma unroll
       for (int i = 0; i < V; ++i) {
-        f[n][i] = in ? f[n][i] - mean : 0.f;
-        s = fmaf(f[n][i], f[n][i], s);
+        xv[n].v[i] = from_f<XT>(0.f);
+        yv[n].v[i] = from_f<YT>(0.f);
+      }
+    }
+    if (SHIFT && (c < 0 || c + V > p.cols)) {
+#pragma unroll
+      for (int i = 0; i < V; ++i)
+        if (outside(c, i)) {
+          xv[n].v[i] = from_f<XT>(0.f);
+          yv[n].v[i] = from_f<YT>(0.f);
+        }
+    }
+  }
+  // 1 / sqrt(mean of squares + eps) of values that are zero outside the row; layer: of the centered values, `mean` theirs
+  auto inverse_norm = [&](auto value, float eps, float& mean) {
+    float s = 0.f;
+    if (LAYER) {
+#pragma unroll
+      for (int n = 0; n < NV; ++n)
+#pragma unroll
+        for (int i = 0; i < V; ++i) s += value(n, i);
+      mean = row_sum<WARP>(s, part, turn) * p.inv_cols;
+      s = 0.f;
+    }
+#pragma unroll
+    for (int n = 0; n < NV; ++n) {
+      const int c = c0 + n * step;
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        float d = value(n, i);
+        if (LAYER) d = (SHIFT ? outside(c, i) : c >= p.cols) ? 0.f : d - mean;
+        s = fmaf(d, d, s);
+      }
+    }
+    return rsqrtf(row_sum<WARP>(s, part, turn) * p.inv_cols + eps);
+  };
+  float f[NV][V];
+  if (p.y != nullptr) {
+    float z_mean = 0.f, z_inv = 1.f;
+    if (p.post_weight != nullptr) z_inv = inverse_norm([&](int n, int i) { return to_f<YT>(yv[n].v[i]); }, p.post_eps, z_mean);
+    const int64_t gate_row = p.gate != nullptr ? static_cast<int64_t>(row_i / p.rows_per_gate) * p.ld_gate : 0;
+    const bool per_col = p.gate != nullptr && p.gate_step != 0;
+    const float row_gate = p.scale * (p.gate != nullptr && !per_col ? to_f<YT>(static_cast<const YT*>(p.gate)[gate_row]) : 1.f);
+#pragma unroll
+    for (int n = 0; n < NV; ++n) {
+      const int c = c0 + n * step;
+      if (c < p.cols) {
+        // f = x + factor * (z - mean) + offset: factor = scale * gate * inverse norm * post weight, offset = scale * gate * post bias
+        float factor[V], w[V];
+#pragma unroll
+        for (int i = 0; i < V; ++i) f[n][i] = to_f<XT>(xv[n].v[i]);
+        if (per_col) {
+          load_vector<YT, V, SHIFT>(p.gate, gate_row, c, p.cols, m, gate_row % 8 == 0, factor);
+          if (p.post_bias != nullptr) {
+            load_vector<YT, V, SHIFT>(p.post_bias, 0, c, p.cols, m, true, w);
+#pragma unroll
+            for (int i = 0; i < V; ++i) f[n][i] = fmaf(p.scale * factor[i], w[i], f[n][i]);
+          }
+          if (p.post_weight != nullptr) {
+            load_vector<YT, V, SHIFT>(p.post_weight, 0, c, p.cols, m, true, w);
+#pragma unroll
+            for (int i = 0; i < V; ++i) factor[i] *= w[i];
+          }
+        } else {
+          if (p.post_bias != nullptr) {
+            load_vector<YT, V, SHIFT>(p.post_bias, 0, c, p.cols, m, true, w);
+#pragma unroll
+            for (int i = 0; i < V; ++i) f[n][i] = fmaf(row_gate, w[i], f[n][i]);
+          }
+          if (p.post_weight != nullptr) {
+            load_vector<YT, V, SHIFT>(p.post_weight, 0, c, p.cols, m, true, factor);
+          } else {
+#pragma unroll
+            for (int i = 0; i < V; ++i) factor[i] = 1.f;
+          }
+        }
+        const float common = (per_col ? p.scale : row_gate) * z_inv;
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+          const float z = to_f<YT>(yv[n].v[i]);
+          f[n][i] = fmaf((LAYER ? z - z_mean : z) * common, factor[i], f[n][i]);
+        }
+        store_piece<XT, V, SHIFT>(p.r, row * p.ld_r + c, c, p.cols, f[n]);
+        if (SHIFT && (c < 0 || c + V > p.cols)) {
+#pragma unroll
+          for (int i = 0; i < V; ++i)
+            if (outside(c, i)) f[n][i] = 0.f;
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < V; ++i) f[n][i] = 0.f;
       }
     }
   } else {
 #pragma unroll
     for (int n = 0; n < NV; ++n)
 #pragma unroll
-      for (int i = 0; i < V; ++i) s = fmaf(f[n][i], f[n][i], s);
-  }
-  const float inv = rsqrtf(block_sum(s, part) * p.inv_cols + eps);
-#pragma unroll
-  for (int n = 0; n < NV; ++n) {
-    const unsigned c = (n * blockDim.x + threadIdx.x) * V;
-    if (c < static_cast<unsigned>(p.cols)) {
-      float w[V], b[V];
-      load_f<YT, V>(weight, c, w);
-      if (bias != nullptr) load_f<YT, V>(bias, c, b);
-#pragma unroll
-      for (int i = 0; i < V; ++i) {
-        f[n][i] = f[n][i] * inv * w[i];
-        if (bias != nullptr) f[n][i] += b[i];
-      }
-    }
-  }
-}
-
-// XT: type of x and r; YT: type of y, h, weights and gate
-template <class XT, class YT, int V, int NV, int MAXT>
-__global__ void __launch_bounds__(MAXT) block_norm_kernel(const NormParams p) {
-  __shared__ float part[32];
-  dependency_wait();
-  dependency_trigger();
-  const int64_t row = blockIdx.x;
-  const unsigned cols = static_cast<unsigned>(p.cols);
-  float f[NV][V], z[NV][V];
-#pragma unroll
-  for (int n = 0; n < NV; ++n) {
-    const unsigned c = (n * blockDim.x + threadIdx.x) * V;
-#pragma unroll
-    for (int i = 0; i < V; ++i) f[n][i] = z[n][i] = 0.f;
-    if (c < cols) {
-      load_f<XT, V>(p.x, row * p.ld_x + c, f[n]);
-      if (p.y != nullptr) load_f<YT, V>(p.y, row * p.ld_y + c, z[n]);
-    }
-  }
-  if (p.y != nullptr) {
-    if (p.post_weight != nullptr) normalise<YT, V, NV>(z, p, p.post_weight, p.post_bias, p.post_eps, part);
-    const int64_t gate_row = p.gate != nullptr ? row / p.rows_per_gate * p.ld_gate : 0;
-    const float row_gate = p.gate != nullptr && p.gate_step == 0 ? to_f<YT>(static_cast<const YT*>(p.gate)[gate_row]) : 1.f;
-#pragma unroll
-    for (int n = 0; n < NV; ++n) {
-      const unsigned c = (n * blockDim.x + threadIdx.x) * V;
-      if (c < cols) {
-        float g[V];
-        const bool per_col = p.gate != nullptr && p.gate_step != 0;
-        if (per_col) load_f<YT, V>(p.gate, gate_row + c, g);
-#pragma unroll
-        for (int i = 0; i < V; ++i) f[n][i] = fmaf(p.scale * (per_col ? g[i] : row_gate), z[n][i], f[n][i]);
-        if (p.r != nullptr) store_f<XT, V>(p.r, row * p.ld_r + c, f[n]);
-      }
-    }
+      for (int i = 0; i < V; ++i) f[n][i] = to_f<XT>(xv[n].v[i]);
   }
   if (p.h == nullptr) return;
-  normalise<YT, V, NV>(f, p, p.weight, p.bias, p.eps, part);
+  float mean = 0.f;
+  const float inv = inverse_norm([&](int n, int i) { return f[n][i]; }, p.eps, mean);
 #pragma unroll
   for (int n = 0; n < NV; ++n) {
-    const unsigned c = (n * blockDim.x + threadIdx.x) * V;
-    if (c < cols) store_f<YT, V>(p.h, row * p.ld_h + c, f[n]);
+    const int c = c0 + n * step;
+    if (c < p.cols) {
+      float w[V];
+      load_vector<YT, V, SHIFT>(p.weight, 0, c, p.cols, m, true, w);
+#pragma unroll
+      for (int i = 0; i < V; ++i) f[n][i] = ((LAYER ? f[n][i] - mean : f[n][i]) * inv) * w[i];
+      if (p.bias != nullptr) {
+        load_vector<YT, V, SHIFT>(p.bias, 0, c, p.cols, m, true, w);
+#pragma unroll
+        for (int i = 0; i < V; ++i) f[n][i] += w[i];
+      }
+      store_piece<YT, V, SHIFT>(p.h, row * p.ld_h + c, c, p.cols, f[n]);
+    }
   }
 }
 
-template <class XT, class YT, int V, int NV>
-int launch_nv(const NormParams& p, int threads, cudaStream_t stream) {
-  if (threads <= 256) return launch_dependent(block_norm_kernel<XT, YT, V, NV, 256>, p.rows, threads, 0, 0, stream, p);
-  return launch_dependent(block_norm_kernel<XT, YT, V, NV, 1024>, p.rows, threads, 0, 0, stream, p);
+template <class XT, class YT, bool SHIFT, bool LAYER>
+int launch_pieces(const NormParams& p, cudaStream_t stream) {
+  const int pieces = (p.cols + (SHIFT ? 14 : 7)) / 8;      // a row may begin at the last value of a piece
+  auto threads = [&](int nv) { return ((pieces + nv - 1) / nv + 31) / 32 * 32; };
+  const int groups = (p.rows + 7) / 8;
+  if (pieces <= 32) return launch_dependent(block_norm_kernel<XT, YT, 8, 1, SHIFT, LAYER, true, 256, 5>, groups, 256, 0, 0, stream, p);
+  if (pieces <= 64) return launch_dependent(block_norm_kernel<XT, YT, 8, 2, SHIFT, LAYER, true, 256, 4>, groups, 256, 0, 0, stream, p);
+  if (pieces <= 512) return launch_dependent(block_norm_kernel<XT, YT, 8, 2, SHIFT, LAYER, false, 256, 4>, p.rows, threads(2), 0, 0, stream, p);
+  if (pieces <= 1024) return launch_dependent(block_norm_kernel<XT, YT, 8, 2, SHIFT, LAYER, false, 512, 2>, p.rows, threads(2), 0, 0, stream, p);
+  return launch_dependent(block_norm_kernel<XT, YT, 8, 4, SHIFT, LAYER, false, 512, 1>, p.rows, threads(4), 0, 0, stream, p);
+}
+template <class XT, class YT, bool LAYER>
+int launch_layer(const NormParams& p, bool vec, bool shift, cudaStream_t stream) {
+  if (vec) return launch_pieces<XT, YT, false, LAYER>(p, stream);
+  if (shift && p.cols <= 16370) return launch_pieces<XT, YT, true, LAYER>(p, stream);
+  if (p.cols <= 1024) return launch_dependent(block_norm_kernel<XT, YT, 1, 4, false, LAYER, false, 256, 1>, p.rows, (p.cols + 127) / 128 * 32, 0, 0, stream, p);
+  return launch_dependent(block_norm_kernel<XT, YT, 1, 16, false, LAYER, false, 1024, 1>, p.rows, (p.cols + 511) / 512 * 32, 0, 0, stream, p);
 }
 template <class XT, class YT>
-int launch_types(const NormParams& p, bool vec, cudaStream_t stream) {
-  const int per = vec ? 8 : 1, pieces = (p.cols + per - 1) / per;
-  auto threads = [&](int nv) { return ((pieces + nv - 1) / nv + 31) / 32 * 32; };
-  if (vec) {
-    if (pieces <= 512) return launch_nv<XT, YT, 8, 1>(p, threads(1), stream);
-    if (pieces <= 2048) return launch_nv<XT, YT, 8, 2>(p, threads(2), stream);
-    return kErrInvalid;
-  }
-  if (pieces <= 1024) return launch_nv<XT, YT, 1, 4>(p, threads(4), stream);
-  if (pieces <= 16384) return launch_nv<XT, YT, 1, 16>(p, threads(16), stream);
-  return kErrInvalid;
+int launch_types(const NormParams& p, bool vec, bool shift, cudaStream_t stream) {
+  return p.layer ? launch_layer<XT, YT, true>(p, vec, shift, stream) : launch_layer<XT, YT, false>(p, vec, shift, stream);
 }
 
 }  // namespace
@@ -211,13 +343,18 @@ int launch_block_norm(const NormArgs& a, cudaStream_t stream) {
                           (gate_vec ? reinterpret_cast<uintptr_t>(a.gate) : 0);
   const int64_t pitches = a.cols | a.ld_x | (a.y ? a.ld_y : 0) | (a.r ? a.ld_r : 0) | (a.h ? a.ld_h : 0) | (gate_vec ? a.ld_gate : 0);
   const bool vec = pitches % 8 == 0 && bases % 16 == 0;
+  // rows of all tensors alike in their pieces: same pitch modulo 8, 16-byte aligned (32 where the values are float)
+  const int64_t pitch = a.ld_x & 7;
+  const bool shift = (!a.y || (a.ld_y & 7) == pitch) && (!a.r || (a.ld_r & 7) == pitch) && (!a.h || (a.ld_h & 7) == pitch) &&
+                     bases % 16 == 0 && ((reinterpret_cast<uintptr_t>(a.x) | reinterpret_cast<uintptr_t>(a.r)) % (a.x_type == 2 ? 32 : 16)) == 0 &&
+                     (a.y_type != 2 || bases % 32 == 0) && (!gate_vec || reinterpret_cast<uintptr_t>(a.gate) % 16 == 0);
   if (a.x_type == 2) {
-    if (a.y_type == 2) return launch_types<float, float>(p, vec, stream);
-    if (a.y_type == kBF16) return launch_types<float, __nv_bfloat16>(p, vec, stream);
-    return launch_types<float, __half>(p, vec, stream);
+    if (a.y_type == 2) return launch_types<float, float>(p, vec, shift, stream);
+    if (a.y_type == kBF16) return launch_types<float, __nv_bfloat16>(p, vec, shift, stream);
+    return launch_types<float, __half>(p, vec, shift, stream);
   }
-  if (a.x_type == kBF16) return launch_types<__nv_bfloat16, __nv_bfloat16>(p, vec, stream);
-  return launch_types<__half, __half>(p, vec, stream);
+  if (a.x_type == kBF16) return launch_types<__nv_bfloat16, __nv_bfloat16>(p, vec, shift, stream);
+  return launch_types<__half, __half>(p, vec, shift, stream);
 }
 
 }  // namespace sfb200
