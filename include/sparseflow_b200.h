@@ -332,7 +332,7 @@ SFB200_API int sfb200_debug_host_chunk_plan(int M, int main_rows, int tail_rows,
  * weighted sum), the norms between two blocks, and low-rank adapters beside a projection.  No counterpart upstream.
  * Everything is decided on the device (group sizes are never read by the host), so each call can be captured into a graph. */
 
-/* Device scratch of sfb200_group_rows above 4096 entries and of sfb200_moe_route above 64 tokens, for that many groups
+/* Device scratch of sfb200_group_rows above 4096 entries and of sfb200_moe_route above 32 tokens, for that many groups
  * (experts); below, workspace may be NULL. */
 SFB200_API size_t sfb200_group_workspace_bytes(int groups);
 

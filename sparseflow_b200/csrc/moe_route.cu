@@ -56,9 +56,9 @@ __device__ __forceinline__ int entry_group(const GroupParams& p, int i, int end)
 
 // The chunk's entries per group into hist[groups].
 __device__ void count_chunk(const GroupParams& p, int begin, int end, int* hist) {
-  for (int g = threadIdx.x; g < p.groups; g += kThreads) hist[g] = 0;
+  for (int g = threadIdx.x; g < p.groups; g += static_cast<int>(blockDim.x)) hist[g] = 0;
   __syncthreads();
-  for (int i0 = begin; i0 < end; i0 += kThreads) {
+  for (int i0 = begin; i0 < end; i0 += static_cast<int>(blockDim.x)) {
     const int g = entry_group(p, i0 + threadIdx.x, end);
     const unsigned same = __match_any_sync(0xffffffffu, g);
     if (g >= 0 && __ffs(same) - 1 == (threadIdx.x & 31)) atomicAdd(&hist[g], __popc(same));
@@ -144,62 +144,86 @@ __device__ __forceinline__ float warp_sum(float v) {
   return v;
 }
 
-// NL: logits per lane
-template <int NL>
+// NL: logits per lane.  NT tokens at a time: the rounds of one token are a chain of reductions, those of two cover each other.
+template <int NL, int NT>
 __device__ void route_tokens(const RouteParams& r, int t_begin, int t_end) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  for (int t = t_begin + warp; t < t_end; t += kWarps) {
-    uint32_t key[NL];
+  const int warps = blockDim.x >> 5;
+  for (int t0 = t_begin + warp; t0 < t_end; t0 += NT * warps) {
+    uint32_t key[NT][NL];
 #pragma unroll
-    for (int i = 0; i < NL; ++i) {
-      const int e = i * 32 + lane;
-      float v = -INFINITY;
-      if (e < r.experts) {
-        const int64_t at = t * r.ld + e;
-        if (r.dtype == 2) v = static_cast<const float*>(r.logits)[at];
-        else if (r.dtype == kBF16) v = __bfloat162float(static_cast<const __nv_bfloat16*>(r.logits)[at]);
-        else v = __half2float(static_cast<const __half*>(r.logits)[at]);
-      }
-      key[i] = order_key(v);
-    }
-    float largest = 0.f, everyone = 0.f, mine = 0.f;      // lane j keeps the j-th choice
-    int expert = -1;
-    for (int j = 0; j < r.top_k; ++j) {
-      uint32_t k = 0;
-      int e = 0x7fffffff;
+    for (int n = 0; n < NT; ++n)
 #pragma unroll
-      for (int i = 0; i < NL; ++i)
-        if (key[i] > k) { k = key[i]; e = i * 32 + lane; }
-      const uint32_t top = __reduce_max_sync(0xffffffffu, k);
-      if (top == 0) break;
-      e = static_cast<int>(__reduce_min_sync(0xffffffffu, k == top ? static_cast<unsigned>(e) : 0x7fffffffu));
-      const float v = key_value(top);
-      if (j == 0) {
-        largest = v;
-        if (!r.renorm) {
-#pragma unroll
-          for (int i = 0; i < NL; ++i)
-            if (key[i] != 0) everyone += expf(key_value(key[i]) - v);
-          everyone = warp_sum(everyone);
+      for (int i = 0; i < NL; ++i) {
+        const int t = t0 + n * warps, e = i * 32 + lane;
+        float v = -INFINITY;
+        if (t < t_end && e < r.experts) {
+          const int64_t at = t * r.ld + e;
+          if (r.dtype == 2) v = static_cast<const float*>(r.logits)[at];
+          else if (r.dtype == kBF16) v = __bfloat162float(static_cast<const __nv_bfloat16*>(r.logits)[at]);
+          else v = __half2float(static_cast<const __half*>(r.logits)[at]);
         }
+        key[n][i] = order_key(v);
       }
-      if (lane == j) { expert = e; mine = expf(v - largest); }
+    float largest[NT], everyone[NT], mine[NT];      // lane j keeps the j-th choice
+    int expert[NT];
 #pragma unroll
-      for (int i = 0; i < NL; ++i)
-        if (i * 32 + lane == e) key[i] = 0;
+    for (int n = 0; n < NT; ++n) {
+      largest[n] = everyone[n] = mine[n] = 0.f;
+      expert[n] = -1;
     }
-    if (r.renorm) everyone = warp_sum(mine);
-    if (lane < r.top_k) {
-      const int64_t at = static_cast<int64_t>(t) * r.top_k + lane;
-      r.weights[at] = expert >= 0 ? mine / everyone : 0.f;
-      r.chosen[at] = expert;
+    for (int j = 0; j < r.top_k; ++j) {
+      uint32_t top[NT];
+      unsigned e[NT];
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        uint32_t k = 0;
+        e[n] = 0x7fffffffu;
+#pragma unroll
+        for (int i = 0; i < NL; ++i)
+          if (key[n][i] > k) { k = key[n][i]; e[n] = i * 32 + lane; }
+        top[n] = __reduce_max_sync(0xffffffffu, k);
+        if (k != top[n]) e[n] = 0x7fffffffu;
+      }
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        if (top[n] == 0) continue;      // nothing left to choose (the whole warp)
+        const int chosen = static_cast<int>(__reduce_min_sync(0xffffffffu, e[n]));
+        const float v = key_value(top[n]);
+        if (j == 0) {
+          largest[n] = v;
+          if (!r.renorm) {
+#pragma unroll
+            for (int i = 0; i < NL; ++i)
+              if (key[n][i] != 0) everyone[n] += expf(key_value(key[n][i]) - v);
+            everyone[n] = warp_sum(everyone[n]);
+          }
+        }
+        if (lane == j) { expert[n] = chosen; mine[n] = expf(v - largest[n]); }
+#pragma unroll
+        for (int i = 0; i < NL; ++i)
+          if (i * 32 + lane == chosen) key[n][i] = 0;
+      }
+    }
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      const int t = t0 + n * warps;
+      if (r.renorm) everyone[n] = warp_sum(mine[n]);
+      if (t < t_end && lane < r.top_k) {
+        const int64_t at = static_cast<int64_t>(t) * r.top_k + lane;
+        r.weights[at] = expert[n] >= 0 ? mine[n] / everyone[n] : 0.f;
+        r.chosen[at] = expert[n];
+      }
     }
   }
 }
 
-// NL = 0: the ids are the caller's.  ONE: a single block does everything; otherwise this launch leaves the blocks' counts.
+// NL = 0: the ids are the caller's.  ONE: a single block does everything; otherwise this launch leaves the blocks' counts, and its blocks
+// are twice as large where the logits of two tokens leave the registers: the choice of a token is latency, and 128 blocks have an SM each.
 template <int NL, bool ONE>
-__global__ void __launch_bounds__(kThreads) group_kernel(const RouteParams r, const GroupParams p) {
+constexpr int group_threads() { return !ONE && NL <= 8 ? 1024 : kThreads; }
+template <int NL, bool ONE>
+__global__ void __launch_bounds__(group_threads<NL, ONE>()) group_kernel(const RouteParams r, const GroupParams p) {
   __shared__ int base[kMaxGroups], hist[kMaxGroups];
   __shared__ uint16_t wcnt[ONE ? kWarps * kMaxGroups : 1];
   dependency_wait();
@@ -210,7 +234,7 @@ __global__ void __launch_bounds__(kThreads) group_kernel(const RouteParams r, co
   if (NL > 0) {
     const int t0 = blockIdx.x * r.tokens_per_block;
     const int t1 = t0 + r.tokens_per_block < r.tokens ? t0 + r.tokens_per_block : r.tokens;
-    route_tokens<NL == 0 ? 1 : NL>(r, t0, t1);
+    route_tokens<NL == 0 ? 1 : NL, NL == 32 ? 1 : 2>(r, t0, t1);
     __syncthreads();
   }
   count_chunk(p, begin, end, hist);
@@ -222,31 +246,30 @@ __global__ void __launch_bounds__(kThreads) group_kernel(const RouteParams r, co
     __syncthreads();
     place_chunk(p, begin, end, base, wcnt);
   } else {
-    for (int g = threadIdx.x; g < p.groups; g += kThreads) p.counts[static_cast<size_t>(blockIdx.x) * p.groups + g] = hist[g];
+    for (int g = threadIdx.x; g < p.groups; g += static_cast<int>(blockDim.x)) p.counts[static_cast<size_t>(blockIdx.x) * p.groups + g] = hist[g];
   }
 }
 
 __global__ void __launch_bounds__(kThreads) place_kernel(const GroupParams p) {
-  __shared__ int base[kMaxGroups], total[kMaxGroups];
+  __shared__ int base[kMaxGroups], total[kMaxGroups], pre[kMaxGroups];
   __shared__ uint16_t wcnt[kWarps * kMaxGroups];
   dependency_wait();
   dependency_trigger();
-  const int me = blockIdx.x;
-  int before[(kMaxGroups + kThreads - 1) / kThreads];
+  const int me = blockIdx.x, blocks = gridDim.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  // a warp adds up the counts of every 16th block, eight blocks' loads at once: one trip to L2 where a thread per group took sixteen
+  for (int g = threadIdx.x; g < p.groups; g += kThreads) total[g] = pre[g] = 0;
+  __syncthreads();
+  for (int g = lane; g < p.groups; g += 32) {
+    int sum = 0, below = 0;
 #pragma unroll
-  for (int j = 0; j < kMaxGroups / kThreads; ++j) {
-    const int g = threadIdx.x + j * kThreads;
-    int sum = 0, pre = 0;
-    if (g < p.groups) {
-#pragma unroll 8
-      for (int b = 0; b < static_cast<int>(gridDim.x); ++b) {
-        const int c = p.counts[static_cast<size_t>(b) * p.groups + g];
-        sum += c;
-        pre += b < me ? c : 0;
-      }
-      total[g] = sum;
+    for (int j = 0; j < kMaxBlocks / kWarps; ++j) {
+      const int b = warp + j * kWarps;
+      const int c = b < blocks ? p.counts[static_cast<size_t>(b) * p.groups + g] : 0;
+      sum += c;
+      below += b < me ? c : 0;
     }
-    before[j] = pre;
+    if (sum) atomicAdd(&total[g], sum);
+    if (below) atomicAdd(&pre[g], below);
   }
   __syncthreads();
   const int all = scan_groups(p.groups, total, base);
@@ -255,11 +278,7 @@ __global__ void __launch_bounds__(kThreads) place_kernel(const GroupParams p) {
     if (threadIdx.x == 0) p.offsets[p.groups] = all;
     __syncthreads();
   }
-#pragma unroll
-  for (int j = 0; j < kMaxGroups / kThreads; ++j) {
-    const int g = threadIdx.x + j * kThreads;
-    if (g < p.groups) base[g] += before[j];
-  }
+  for (int g = threadIdx.x; g < p.groups; g += kThreads) base[g] += pre[g];
   __syncthreads();
   const int64_t begin64 = static_cast<int64_t>(me) * p.chunk;
   const int begin = static_cast<int>(begin64 < p.n ? begin64 : p.n);
@@ -271,7 +290,7 @@ __global__ void __launch_bounds__(kThreads) place_kernel(const GroupParams p) {
 template <int NL>
 int launch_group(const RouteParams& r, const GroupParams& p, int blocks, cudaStream_t stream) {
   if (blocks == 1) return launch_dependent(group_kernel<NL, true>, 1, kThreads, 0, 0, stream, r, p);
-  const int rc = launch_dependent(group_kernel<NL, false>, blocks, kThreads, 0, 0, stream, r, p);
+  const int rc = launch_dependent(group_kernel<NL, false>, blocks, group_threads<NL, false>(), 0, 0, stream, r, p);
   if (rc != kOk) return rc;
   return launch_dependent(place_kernel, blocks, kThreads, 0, 0, stream, p);
 }
@@ -297,9 +316,10 @@ int launch_moe_route(const RouteArgs& a, cudaStream_t stream) {
   if (a.tokens > 0 && (!a.logits || !a.weights || !a.chosen || !a.rows || !a.slots)) return kErrInvalid;
   if (static_cast<int64_t>(a.tokens) * a.top_k > 0x7fffffffll - kThreads) return kErrInvalid;
   const int n = a.tokens * a.top_k;
-  // to 64 tokens one block (four tokens a warp) costs less than a second launch; beyond, 16 tokens a block or more
+  // to 32 tokens one block (two tokens a warp) costs less than a second launch (6.2 us; 64 tokens 9.8 us, in two launches 6.6); beyond, 16 tokens a
+  // block or more
   int per_block = a.tokens;
-  if (a.tokens > 64) {
+  if (a.tokens > 32) {
     per_block = (a.tokens + kMaxBlocks - 1) / kMaxBlocks;
     if (per_block < kWarps) per_block = kWarps;
   }

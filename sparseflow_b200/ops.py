@@ -9,6 +9,7 @@ sites (sparseflow/fused_mlp.py:54,60; sparseflow/nn/sparseflow_linear.py:123) an
 from __future__ import annotations
 
 import ctypes as C
+import functools
 from dataclasses import dataclass
 from typing import Optional
 
@@ -279,6 +280,29 @@ def force_token_tile(bn: int) -> None:
 # none of these calls waits for the GPU, and each can be captured into a CUDA graph.
 
 _DT3 = {torch.float16: 0, torch.bfloat16: 1, torch.float32: 2}
+_current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
+
+
+def _stream_of(dev: int) -> int:
+    return _raw_stream(dev) if _raw_stream is not None else torch.cuda.current_stream(dev).cuda_stream
+
+
+def _on_own_device(fn):
+    """The call with its first tensor's device current.  One comparison where it already is: a context manager costs a microsecond, and
+    these calls are launched eagerly around kernels of a few."""
+    first = fn.__code__.co_varnames[0]
+
+    @functools.wraps(fn)
+    def call(*args, **kw):
+        t = args[0] if args else kw[first]
+        if not t.is_cuda:
+            raise ValueError(f"{first} must be a CUDA tensor")
+        dev = t.get_device()
+        if dev == _current_device():
+            return fn(*args, **kw)
+        with torch.cuda.device(dev):
+            return fn(*args, **kw)
+    return call
 
 
 def _on_device_of(x: torch.Tensor, t: Optional[torch.Tensor], name: str) -> None:
@@ -313,6 +337,18 @@ def _check_out(out: torch.Tensor, like: torch.Tensor, shape: tuple, dtype: torch
         raise ValueError(f"out must be {shape} {dtype} on {like.device}")
     if (out.stride(-1) != 1 and shape[-1] > 1) or (out.dim() == 2 and shape[0] > 1 and out.stride(0) < shape[1]):
         raise ValueError("out must have unit inner stride and rows that do not overlap")
+
+
+def _extent(t: torch.Tensor) -> tuple:
+    n = sum((d - 1) * s for d, s in zip(t.shape, t.stride())) + 1 if t.numel() else 0
+    return t.data_ptr(), t.data_ptr() + n * t.element_size()
+
+
+def _check_apart(out: torch.Tensor, t: torch.Tensor, name: str, same: bool = False) -> None:
+    """The kernels read ``t`` while they write ``out``: the two share no memory, or (``same``) are the same rows."""
+    (a, b), (c, d) = _extent(out), _extent(t)
+    if a < d and c < b and not (same and a == c and out.shape == t.shape and _pitch(out) == _pitch(t)):
+        raise ValueError(f"out and {name} share memory")
 
 
 @dataclass
@@ -360,36 +396,31 @@ def group_rows(ids: torch.Tensor, groups: int, per_row: int = 1) -> RowGroups:
     return RowGroups(offsets, rows, slots, groups, per_row)
 
 
+@_on_own_device
 def moe_route(logits: torch.Tensor, top_k: int, renormalize: bool = True) -> Routing:
     """Route tokens to experts: the ``top_k`` largest of ``logits[tokens, experts]`` (ties to the lowest expert), their softmax
     weights (over all experts, or with ``renormalize`` over the chosen ones), and the grouping of the tokens by expert.
 
     A logit of -inf or NaN is never chosen; a token with fewer than ``top_k`` others gets expert -1 with weight 0 there (a row of
     padding, all -inf, goes nowhere).  +inf counts as the largest finite number."""
-    if not logits.is_cuda:
-        raise ValueError("logits must be a CUDA tensor")
     dt = _DT3.get(logits.dtype)
     if dt is None:
         raise ValueError(f"logits must be float16, bfloat16 or float32, got {logits.dtype}")
-    if logits.dim() != 2:
-        raise ValueError(f"logits must be 2D, got {logits.dim()}D")
+    logits = _rows2d(logits, "logits")
     n, E = logits.shape
     if not 1 <= E <= 1024:
         raise ValueError(f"experts must be 1 .. 1024, got {E}")
     if not 1 <= top_k <= min(32, E):
         raise ValueError(f"top_k must be 1 .. {min(32, E)}, got {top_k}")
-    logits = _rows2d(logits, "logits")
-    dev = logits.device
     L = _lib.lib()
-    with _on(dev):
-        weights = torch.empty((n, top_k), dtype=torch.float32, device=dev)
-        chosen = torch.empty((n, top_k), dtype=torch.int32, device=dev)
-        slots = torch.empty((n, top_k), dtype=torch.int32, device=dev)
-        rows = torch.empty(n * top_k, dtype=torch.int32, device=dev)
-        offsets = torch.empty(E + 1, dtype=torch.int32, device=dev)
-        work = torch.empty(L.sfb200_group_workspace_bytes(E), dtype=torch.uint8, device=dev) if n > 64 else None
-        rc = L.sfb200_moe_route(logits.data_ptr(), _pitch(logits), n, E, top_k, dt, 1 if renormalize else 0, weights.data_ptr(), chosen.data_ptr(),
-                                offsets.data_ptr(), rows.data_ptr(), slots.data_ptr(), _ptr(work), _stream())
+    weights = logits.new_empty((n, top_k), dtype=torch.float32)
+    chosen = logits.new_empty((n, top_k), dtype=torch.int32)
+    slots = logits.new_empty((n, top_k), dtype=torch.int32)
+    rows = logits.new_empty(n * top_k, dtype=torch.int32)
+    offsets = logits.new_empty(E + 1, dtype=torch.int32)
+    work = logits.new_empty(L.sfb200_group_workspace_bytes(E), dtype=torch.uint8) if n > 32 else None
+    rc = L.sfb200_moe_route(logits.data_ptr(), _pitch(logits), n, E, top_k, dt, 1 if renormalize else 0, weights.data_ptr(), chosen.data_ptr(),
+                            offsets.data_ptr(), rows.data_ptr(), slots.data_ptr(), _ptr(work), _stream_of(logits.get_device()))
     if rc:
         _lib.check("sfb200_moe_route", rc)
     return Routing(weights, chosen, RowGroups(offsets, rows, slots, E, top_k))
@@ -474,8 +505,6 @@ def _expert_bias(b: Optional[torch.Tensor], x: torch.Tensor, experts: int, cols:
 
 
 def _grouped_args(x: torch.Tensor, cw: CompressedExperts, groups: RowGroups, gather: bool):
-    if not x.is_cuda:
-        raise ValueError("x must be a CUDA tensor")
     if x.dim() != 2 or x.shape[1] != cw.K:
         raise ValueError(f"Expected last dim {cw.K}, got {tuple(x.shape)}")
     if x.dtype != cw.dtype:
@@ -498,34 +527,36 @@ def _grouped_scratch(x: torch.Tensor, total: int, cw: CompressedExperts) -> Opti
     return torch.empty(n, dtype=torch.uint8, device=x.device) if n else None
 
 
+@_on_own_device
 def grouped_sparse_gemm(x: torch.Tensor, cw: CompressedExperts, groups: RowGroups, bias: Optional[torch.Tensor] = None, act: Optional[str] = None,
                         gather: bool = False, out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """y[place] = act(x[place] . W_e^T + bias[e]) for the places of every expert e.
 
     ``x`` holds a row per place in the order of ``groups``; with ``gather`` a row per token, read through ``groups.rows``.  Rows of the
-    result behind the last group are left as they were (in a fresh result: undefined)."""
+    result behind the last group are left as they were (in a fresh result: undefined).  ``out`` shares no memory with ``x``."""
     x, total = _grouped_args(x, cw, groups, gather)
     if act not in ACT:
         raise ValueError(f"unknown activation {act!r}")
     if cw.gate_up:
         raise ValueError("gate|up weights: use grouped_sparse_gemm_swiglu")
     bias = _expert_bias(bias, x, cw.experts, cw.rows, "bias")
-    with _on(x.device):
-        if out is None:
-            out = x.new_empty((total, cw.rows))
-        else:
-            _check_out(out, x, (total, cw.rows), x.dtype)
-        if total == 0:
-            return out
-        scratch = _grouped_scratch(x, total, cw) if gather else None
-        rc = _lib.lib().sfb200_grouped_sparse_gemm(x.data_ptr(), _pitch(x), x.shape[0], groups.rows.data_ptr() if gather else None, _ptr(scratch),
-                                                   cw.values.data_ptr(), cw.meta.data_ptr(), out.data_ptr(), _pitch(out), total, cw.experts, cw.rows,
-                                                   cw.K, _dt(x), _ptr(bias), ACT[act], groups.offsets.data_ptr(), _stream())
+    if out is None:
+        out = x.new_empty((total, cw.rows))
+    else:
+        _check_out(out, x, (total, cw.rows), x.dtype)
+        _check_apart(out, x, "x")
+    if total == 0:
+        return out
+    scratch = _grouped_scratch(x, total, cw) if gather else None
+    rc = _lib.lib().sfb200_grouped_sparse_gemm(x.data_ptr(), _pitch(x), x.shape[0], groups.rows.data_ptr() if gather else None, _ptr(scratch),
+                                               cw.values.data_ptr(), cw.meta.data_ptr(), out.data_ptr(), _pitch(out), total, cw.experts, cw.rows,
+                                               cw.K, _dt(x), _ptr(bias), ACT[act], groups.offsets.data_ptr(), _stream_of(x.get_device()))
     if rc:
         _lib.check("sfb200_grouped_sparse_gemm", rc)
     return out
 
 
+@_on_own_device
 def grouped_sparse_gemm_swiglu(x: torch.Tensor, cw_gu: CompressedExperts, groups: RowGroups, gather: bool = False,
                                gate_bias: Optional[torch.Tensor] = None, up_bias: Optional[torch.Tensor] = None,
                                out: Optional[torch.Tensor] = None) -> torch.Tensor:
@@ -537,28 +568,28 @@ def grouped_sparse_gemm_swiglu(x: torch.Tensor, cw_gu: CompressedExperts, groups
     I = cw_gu.rows // 2
     gate_bias = _expert_bias(gate_bias, x, cw_gu.experts, I, "gate_bias")
     up_bias = _expert_bias(up_bias, x, cw_gu.experts, I, "up_bias")
-    with _on(x.device):
-        if out is None:
-            out = x.new_empty((total, I))
-        else:
-            _check_out(out, x, (total, I), x.dtype)
-        if total == 0:
-            return out
-        scratch = _grouped_scratch(x, total, cw_gu) if gather else None
-        rc = _lib.lib().sfb200_grouped_sparse_gemm_swiglu(x.data_ptr(), _pitch(x), x.shape[0], groups.rows.data_ptr() if gather else None,
-                                                          _ptr(scratch), cw_gu.values.data_ptr(), cw_gu.meta.data_ptr(), out.data_ptr(), _pitch(out),
-                                                          total, cw_gu.experts, I, cw_gu.K, _dt(x), _ptr(gate_bias), _ptr(up_bias),
-                                                          groups.offsets.data_ptr(), _stream())
+    if out is None:
+        out = x.new_empty((total, I))
+    else:
+        _check_out(out, x, (total, I), x.dtype)
+        _check_apart(out, x, "x")
+    if total == 0:
+        return out
+    scratch = _grouped_scratch(x, total, cw_gu) if gather else None
+    rc = _lib.lib().sfb200_grouped_sparse_gemm_swiglu(x.data_ptr(), _pitch(x), x.shape[0], groups.rows.data_ptr() if gather else None,
+                                                      _ptr(scratch), cw_gu.values.data_ptr(), cw_gu.meta.data_ptr(), out.data_ptr(), _pitch(out),
+                                                      total, cw_gu.experts, I, cw_gu.K, _dt(x), _ptr(gate_bias), _ptr(up_bias),
+                                                      groups.offsets.data_ptr(), _stream_of(x.get_device()))
     if rc:
         _lib.check("sfb200_grouped_sparse_gemm_swiglu", rc)
     return out
 
 
+@_on_own_device
 def moe_combine(y: torch.Tensor, slots: torch.Tensor, weights: torch.Tensor, residual: Optional[torch.Tensor] = None,
                 out: Optional[torch.Tensor] = None) -> torch.Tensor:
-    """out[t] = residual[t] + sum_j weights[t, j] * y[slots[t, j]], in 32 bits, rounded once; a slot of -1 adds nothing."""
-    if not y.is_cuda:
-        raise ValueError("y must be a CUDA tensor")
+    """out[t] = residual[t] + sum_j weights[t, j] * y[slots[t, j]], in 32 bits, rounded once; a slot of -1 adds nothing.
+    ``out`` may be ``residual``."""
     dt = _dt(y)
     y = _rows2d(y, "y")
     if slots.dim() != 2 or slots.shape != weights.shape or slots.dtype != torch.int32 or weights.dtype != torch.float32 or not slots.shape[1]:
@@ -577,18 +608,21 @@ def moe_combine(y: torch.Tensor, slots: torch.Tensor, weights: torch.Tensor, res
         residual = _rows2d(residual, "residual")
         ld_res = _pitch(residual)
     slots, weights = slots.contiguous(), weights.contiguous()
-    with _on(y.device):
-        if out is None:
-            out = y.new_empty((n, H))
-        else:
-            _check_out(out, y, (n, H), y.dtype)
-        rc = _lib.lib().sfb200_moe_combine(y.data_ptr(), _pitch(y), y.shape[0], slots.data_ptr(), weights.data_ptr(), _ptr(residual), ld_res,
-                                           out.data_ptr(), _pitch(out), n, k, H, dt, _stream())
+    if out is None:
+        out = y.new_empty((n, H))
+    else:
+        _check_out(out, y, (n, H), y.dtype)
+        _check_apart(out, y, "y")
+        if residual is not None:
+            _check_apart(out, residual, "residual", same=True)
+    rc = _lib.lib().sfb200_moe_combine(y.data_ptr(), _pitch(y), y.shape[0], slots.data_ptr(), weights.data_ptr(), _ptr(residual), ld_res,
+                                       out.data_ptr(), _pitch(out), n, k, H, dt, _stream_of(y.get_device()))
     if rc:
         _lib.check("sfb200_moe_combine", rc)
     return out
 
 
+@_on_own_device
 def block_norm(x: torch.Tensor, y: Optional[torch.Tensor] = None, *, weight: Optional[torch.Tensor], bias: Optional[torch.Tensor] = None,
                post_weight: Optional[torch.Tensor] = None, post_bias: Optional[torch.Tensor] = None, gate: Optional[torch.Tensor] = None,
                scale: float = 1.0, eps: float = 1e-5, post_eps: Optional[float] = None, kind: str = "rms"):
@@ -601,8 +635,6 @@ def block_norm(x: torch.Tensor, y: Optional[torch.Tensor] = None, *, weight: Opt
     ``kind``: "rms" or "layer".  ``x`` [rows, cols] float16, bfloat16 or float32; ``y``, the weights, the gate and ``h`` have one
     type, that of ``x`` or (``x`` float32) a 16-bit one.  ``gate``: [cols]; or [g, cols] / [g, 1], each row for rows / g consecutive
     rows.  Without ``y``: r is ``x`` itself.  ``weight=None`` (with ``y``): no second norm, h is None."""
-    if not x.is_cuda:
-        raise ValueError("x must be a CUDA tensor")
     if kind not in ("rms", "layer"):
         raise ValueError(f"kind must be 'rms' or 'layer', got {kind!r}")
     xt = _DT3.get(x.dtype)
@@ -632,7 +664,11 @@ def block_norm(x: torch.Tensor, y: Optional[torch.Tensor] = None, *, weight: Opt
             raise ValueError(f"{name} must be [{H}] {dtype}, got {tuple(v.shape)} {v.dtype}")
         return v if v.is_contiguous() else v.contiguous()
 
-    weight, bias, post_weight, post_bias = vector(weight, "weight"), vector(bias, "bias"), vector(post_weight, "post_weight"), vector(post_bias, "post_bias")
+    weight = vector(weight, "weight")
+    if bias is not None:
+        bias = vector(bias, "bias")
+    if post_weight is not None:
+        post_weight, post_bias = vector(post_weight, "post_weight"), vector(post_bias, "post_bias")
     ld_y = ld_gate = gate_rows = gate_cols = 0
     if y is not None:
         _on_device_of(x, y, "y")
@@ -650,12 +686,11 @@ def block_norm(x: torch.Tensor, y: Optional[torch.Tensor] = None, *, weight: Opt
             raise ValueError(f"gate must be [{H}], or [g, {H}] or [g, 1] with g dividing {n} rows, got {tuple(gate.shape)}")
         gate = _rows2d(gate, "gate")
         ld_gate, (gate_rows, gate_cols) = _pitch(gate), gate.shape
-    with _on(x.device):
-        r = torch.empty((n, H), dtype=x.dtype, device=x.device) if y is not None else None
-        h = torch.empty((n, H), dtype=dtype, device=x.device) if weight is not None else None
-        rc = _lib.lib().sfb200_block_norm(x.data_ptr(), _pitch(x), _ptr(y), ld_y, _ptr(weight), _ptr(bias), _ptr(post_weight), _ptr(post_bias), _ptr(gate),
-                                          ld_gate, gate_rows, gate_cols, _ptr(r), H, _ptr(h), H, n, H, xt, yt, scale, eps,
-                                          eps if post_eps is None else post_eps, 1 if kind == "layer" else 0, _stream())
+    r = x.new_empty((n, H)) if y is not None else None
+    h = (x if y is None else y).new_empty((n, H), dtype=dtype) if weight is not None else None
+    rc = _lib.lib().sfb200_block_norm(x.data_ptr(), _pitch(x), _ptr(y), ld_y, _ptr(weight), _ptr(bias), _ptr(post_weight), _ptr(post_bias), _ptr(gate),
+                                      ld_gate, gate_rows, gate_cols, _ptr(r), H, _ptr(h), H, n, H, xt, yt, scale, eps,
+                                      eps if post_eps is None else post_eps, 1 if kind == "layer" else 0, _stream_of(x.get_device()))
     if rc:
         _lib.check("sfb200_block_norm", rc)
     return (x if r is None else r), h
@@ -706,11 +741,10 @@ def _kernel_ready_bank(t: torch.Tensor) -> torch.Tensor:
     return t if t.data_ptr() % 16 == 0 else t.clone()
 
 
+@_on_own_device
 def lora_add(y: torch.Tensor, x: torch.Tensor, bank: LoraBank, groups: RowGroups, out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """out[t] = y[t] + scale_g * (x[t] . A_g^T) . B_g^T for the rows of adapter g (``groups = group_rows(ids, bank.adapters)``); rows of
     no adapter keep ``y``.  ``out`` may be ``y``."""
-    if not y.is_cuda:
-        raise ValueError("y must be a CUDA tensor")
     n = x.shape[0]
     if x.dim() != 2 or x.shape[1] != bank.K or tuple(y.shape) != (n, bank.N):
         raise ValueError(f"expected x [rows, {bank.K}] and y [rows, {bank.N}], got {tuple(x.shape)} and {tuple(y.shape)}")
@@ -722,27 +756,28 @@ def lora_add(y: torch.Tensor, x: torch.Tensor, bank: LoraBank, groups: RowGroups
     _on_device_of(y, bank.a, "adapters")
     _on_device_of(y, groups.offsets, "groups")
     x = _rows16(x, "x")
-    with _on(y.device):
-        if out is None:
+    if out is None:
+        out = y.new_empty((n, bank.N))
+    else:
+        _check_out(out, y, (n, bank.N), y.dtype)
+        _check_apart(out, x, "x")
+        _check_apart(out, y, "y", same=True)
+    if n == 0:
+        return out
+    into = out
+    if out is y:
+        y = out = _rows16(y, "y")
+    else:
+        y = _rows16(y, "y")
+        if out.data_ptr() % 16 or _pitch(out) % 8:
             out = y.new_empty((n, bank.N))
-        elif out is not y:
-            _check_out(out, y, (n, bank.N), y.dtype)
-        if n == 0:
-            return out
-        into = out
-        if out is y:
-            y = out = _rows16(y, "y")
-        else:
-            y = _rows16(y, "y")
-            if out.data_ptr() % 16 or _pitch(out) % 8:
-                out = y.new_empty((n, bank.N))
-        L = _lib.lib()
-        work = torch.empty(L.sfb200_lora_workspace_bytes(n, bank.rank), dtype=torch.uint8, device=y.device)
-        rc = L.sfb200_lora_add(y.data_ptr(), _pitch(y), x.data_ptr(), _pitch(x), bank.a.data_ptr(), bank.b.data_ptr(), bank.scales.data_ptr(),
-                                        out.data_ptr(), _pitch(out), n, bank.adapters, bank.rank, bank.K, bank.N, _dt(y), groups.offsets.data_ptr(),
-                                        groups.rows.data_ptr(), groups.slots.data_ptr(), work.data_ptr(), _stream())
-        if rc:
-            _lib.check("sfb200_lora_add", rc)
-        if out is not into:
-            into.copy_(out)
+    L = _lib.lib()
+    work = y.new_empty(L.sfb200_lora_workspace_bytes(n, bank.rank), dtype=torch.uint8)
+    rc = L.sfb200_lora_add(y.data_ptr(), _pitch(y), x.data_ptr(), _pitch(x), bank.a.data_ptr(), bank.b.data_ptr(), bank.scales.data_ptr(),
+                           out.data_ptr(), _pitch(out), n, bank.adapters, bank.rank, bank.K, bank.N, _dt(y), groups.offsets.data_ptr(),
+                           groups.rows.data_ptr(), groups.slots.data_ptr(), work.data_ptr(), _stream_of(y.get_device()))
+    if rc:
+        _lib.check("sfb200_lora_add", rc)
+    if out is not into:
+        into.copy_(out)
     return into
