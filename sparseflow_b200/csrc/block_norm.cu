@@ -321,11 +321,11 @@ int launch_types(const NormParams& p, bool vec, bool shift, cudaStream_t stream)
 
 int launch_block_norm(const NormArgs& a, cudaStream_t stream) {
   if (a.rows < 0 || a.cols < 1 || a.cols > kNormMaxCols) return kErrInvalid;
+  if (a.rows == 0) return kOk;
   if (!a.x || (!a.r && !a.h) || (a.h && !a.weight) || (a.y && !a.r) || (!a.y && (a.r || a.gate || a.post_weight))) return kErrInvalid;
   if (a.ld_x < a.cols || (a.y && a.ld_y < a.cols) || (a.r && a.ld_r < a.cols) || (a.h && a.ld_h < a.cols)) return kErrInvalid;
   if (a.gate && (a.gate_rows < 1 || a.rows % a.gate_rows != 0 || (a.gate_cols != 1 && a.gate_cols != a.cols))) return kErrInvalid;
   if (a.x_type < 0 || a.x_type > 2 || a.y_type < 0 || a.y_type > 2 || (a.x_type != a.y_type && a.x_type != 2)) return kErrInvalid;
-  if (a.rows == 0) return kOk;
   NormParams p{};
   p.x = a.x; p.y = a.y; p.weight = a.weight; p.bias = a.bias; p.post_weight = a.post_weight; p.post_bias = a.post_bias;
   p.gate = a.gate; p.r = a.r; p.h = a.h;

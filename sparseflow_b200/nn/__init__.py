@@ -1,6 +1,6 @@
 """sparseflow_b200.nn: the module-level surface of the reference's ``sparseflow.nn`` (its ``__init__`` exports
 ``SparseFlowPolicy``, ``replace_llama_mlp_module``, the Linear and MLP classes and their ``make_*`` helpers,
-sparseflow/nn/__init__.py:12-27) plus ``SparseLinear`` and the ``replace_llama*`` helpers.
+sparseflow/nn/__init__.py:12-27) plus ``SparseLinear``, the ``replace_llama*`` helpers, ``SparseFlowMoE`` and ``SparseFlowBlockNorm``.
 
 Like upstream, importing the package must never fail because one submodule cannot be imported (torch missing, the CUDA
 library not built yet): each name is bound only if its module imports and defines it.
@@ -12,6 +12,8 @@ _EXPORTS = {
     "surgery": ("replace_llama_mlp_module",),
     "sparseflow_linear": ("SparseFlowLinear", "make_sparseflow_linear", "prune_24_dense_weight"),
     "sparseflow_mlp": ("SparseFlowMLP", "make_sparseflow_mlp"),
+    "sparseflow_moe": ("SparseFlowMoE", "make_sparseflow_moe"),
+    "block_norm": ("SparseFlowBlockNorm",),
     "sparse_linear": ("SparseLinear",),
     "replace_llama": ("replace_llama_mlp", "replace_llama_full", "replace_llama_attention"),
 }

@@ -10,6 +10,8 @@ Interface of the reference's ``sparseflow/nn/sparseflow_linear.py``: ``prune_24_
   the reference's ``torch.topk`` leaves tie order unspecified;
 * bias is applied in the GEMM epilogue, and no transpose / ``.contiguous()`` copy of the output is
   needed (the reference computes Y^T and copies, :121-124);
+* low-rank adapters of many requests at once beside the shared weight: ``set_adapters(bank)``, then ``forward(x, adapters)`` with the rows
+  grouped by adapter (``ops.group_rows``); they are added to the output of either branch;
 * the dense branch uses the ORIGINAL weight, as upstream does (:128-130); pass
   ``dense_uses_pruned=True`` to make both branches compute the same function.
 """
@@ -92,6 +94,22 @@ class SparseFlowLinear(nn.Module):
 
         self._sparse_count = 0
         self._dense_count = 0
+        self.adapters: Optional[ops.LoraBank] = None
+
+    def set_adapters(self, bank: Optional[ops.LoraBank]) -> None:
+        """The low-rank adapters that ``forward`` adds for the rows grouped to them; None removes them."""
+        if bank is not None and (bank.K, bank.N, bank.dtype) != (self.in_features, self.out_features, self.W_original.dtype):
+            raise ValueError(f"adapters are {bank.K} -> {bank.N} {bank.dtype}, the layer {self.in_features} -> {self.out_features} {self.W_original.dtype}")
+        if bank is not None and bank.a.device != self.W_original.device:
+            raise ValueError(f"adapters are on {bank.a.device}, the layer on {self.W_original.device}")
+        self.adapters = bank
+
+    def _adapt(self, y2d: torch.Tensor, x2d: torch.Tensor, groups: Optional[ops.RowGroups]) -> torch.Tensor:
+        if groups is None:
+            return y2d
+        if self.adapters is None:
+            raise ValueError("rows are grouped by adapter but the layer has none: call set_adapters")
+        return ops.lora_add(y2d, x2d, self.adapters, groups, out=y2d)
 
     @property
     def W_sparse(self) -> Optional[ops.Compressed24]:
@@ -105,7 +123,7 @@ class SparseFlowLinear(nn.Module):
             f"sparse_weight={self._supports_sparse_weight}"
         )
 
-    def forward(self, x: torch.Tensor) -> torch.Tensor:
+    def forward(self, x: torch.Tensor, adapters: Optional[ops.RowGroups] = None) -> torch.Tensor:
         _require_cuda_16bit(x, "x")
         if x.shape[-1] != self.in_features:
             raise ValueError(f"Expected last dim {self.in_features}, got {x.shape[-1]}")
@@ -121,12 +139,14 @@ class SparseFlowLinear(nn.Module):
         # itself (its output is a fresh tensor), so only the library GEMM needs no_grad.
         if use_sparse:
             self.__dict__["_sparse_count"] += 1
-            y2d = ops.sparse_gemm(x.reshape(M, self.in_features), self.W_sparse, bias=self.bias)
+            x2d = x.reshape(M, self.in_features)
+            y2d = self._adapt(ops.sparse_gemm(x2d, self.W_sparse, bias=self.bias), x2d, adapters)
             return y2d.view(*leading, self.out_features)
         with torch.no_grad():
             self.__dict__["_dense_count"] += 1
             W = self.W_dense_pruned if self.dense_uses_pruned else self.W_original
-            y2d = F.linear(x.reshape(M, self.in_features), W, self.bias)
+            x2d = x.reshape(M, self.in_features)
+            y2d = self._adapt(F.linear(x2d, W, self.bias), x2d, adapters)
             return y2d.reshape(*leading, self.out_features)
 
     @property

@@ -1,0 +1,109 @@
+"""``SparseFlowMoE``: a mixture of gated experts over 2:4 weights.
+
+    p = router(x), the top_k experts of every token; out = sum_j p_j * down_e(silu(gate_e(x)) * up_e(x))   (+ residual)
+
+The experts' weights are pruned and compressed once; a forward pass is the router's product, ``moe_route``, one grouped gate|up
+product that reads the tokens through the grouping and applies SiLU.mul, one grouped down product, and ``moe_combine``.  Group sizes
+stay on the device, so the pass never waits for the GPU and can be captured into a CUDA graph.  No counterpart upstream, whose gated FFN
+(sparseflow/nn/sparseflow_mlp.py:15-130) is one expert; interface and error behaviour follow ``SparseFlowMLP``.
+"""
+from __future__ import annotations
+
+from typing import Optional
+
+import torch
+import torch.nn as nn
+import torch.nn.functional as F
+
+from .. import ops
+
+
+class SparseFlowMoE(nn.Module):
+    """``router_weight`` [experts, hidden] (any float type: the router runs in it); ``gate_weight`` / ``up_weight`` [experts, intermediate,
+    hidden], ``down_weight`` [experts, hidden, intermediate] float16 or bfloat16 on CUDA; biases [experts, features] or None.
+    ``renormalize``: the weights of a token's experts sum to one."""
+
+    def __init__(
+        self,
+        router_weight: torch.Tensor,
+        gate_weight: torch.Tensor,
+        up_weight: torch.Tensor,
+        down_weight: torch.Tensor,
+        top_k: int,
+        renormalize: bool = True,
+        gate_bias: Optional[torch.Tensor] = None,
+        up_bias: Optional[torch.Tensor] = None,
+        down_bias: Optional[torch.Tensor] = None,
+        router_bias: Optional[torch.Tensor] = None,
+    ):
+        super().__init__()
+        if gate_weight.dim() != 3:
+            raise ValueError(f"gate_weight must be [experts, intermediate, hidden], got {gate_weight.dim()}D")
+        E, I, H = gate_weight.shape
+        if up_weight.shape != gate_weight.shape or tuple(down_weight.shape) != (E, H, I):
+            raise ValueError(f"gate {tuple(gate_weight.shape)}, up {tuple(up_weight.shape)} and down {tuple(down_weight.shape)} do not form experts")
+        if tuple(router_weight.shape) != (E, H):
+            raise ValueError(f"router_weight must be [{E}, {H}], got {tuple(router_weight.shape)}")
+        if not 1 <= top_k <= min(32, E):
+            raise ValueError(f"top_k must be 1 .. {min(32, E)}, got {top_k}")
+        if H % 64 or I % 64:
+            raise ValueError(f"hidden and intermediate size must be multiples of 64, got {H} and {I}")
+        self.experts, self.hidden_size, self.intermediate_size = E, H, I
+        self.top_k, self.renormalize = int(top_k), bool(renormalize)
+        gu = ops.compress_gate_up_experts(gate_weight.detach(), up_weight.detach())
+        down = ops.compress_experts(down_weight.detach())
+        for name, t in (("router_weight", router_weight), ("router_bias", router_bias), ("gu_values", gu.values), ("gu_meta", gu.meta),
+                        ("down_values", down.values), ("down_meta", down.meta), ("gate_bias", gate_bias), ("up_bias", up_bias), ("down_bias", down_bias)):
+            self.register_buffer(name, None if t is None else t.detach().contiguous(), persistent=False)
+
+    def _weights(self):
+        E, H, I = self.experts, self.hidden_size, self.intermediate_size
+        return (ops.CompressedExperts(self.gu_values, self.gu_meta, E, 2 * I, H, gate_up=True),
+                ops.CompressedExperts(self.down_values, self.down_meta, E, H, I))
+
+    def route(self, x2d: torch.Tensor) -> ops.Routing:
+        logits = F.linear(x2d.to(self.router_weight.dtype), self.router_weight, self.router_bias)
+        return ops.moe_route(logits, self.top_k, renormalize=self.renormalize)
+
+    @torch.no_grad()
+    def forward(self, x: torch.Tensor, residual: Optional[torch.Tensor] = None) -> torch.Tensor:
+        if x.shape[-1] != self.hidden_size:
+            raise ValueError(f"Expected last dim {self.hidden_size}, got {x.shape[-1]}")
+        x2d = x.reshape(-1, self.hidden_size)
+        routing = self.route(x2d)
+        gu, down = self._weights()
+        hidden = ops.grouped_sparse_gemm_swiglu(x2d, gu, routing.groups, gather=True, gate_bias=self.gate_bias, up_bias=self.up_bias)
+        y = ops.grouped_sparse_gemm(hidden, down, routing.groups, bias=self.down_bias)
+        out = ops.moe_combine(y, routing.groups.slots, routing.weights, residual=None if residual is None else residual.reshape(-1, self.hidden_size))
+        return out.view(*x.shape)
+
+
+def _stacked(linears, what: str):
+    weights = torch.stack([m.weight.detach() for m in linears])
+    biases = [getattr(m, "bias", None) for m in linears]
+    if any(b is None for b in biases) != all(b is None for b in biases):
+        raise ValueError(f"some experts' {what} projections have a bias and some have none")
+    return weights, None if biases[0] is None else torch.stack([b.detach() for b in biases])
+
+
+def is_moe(module: nn.Module) -> bool:
+    """Whether a module has the layout ``make_sparseflow_moe`` reads."""
+    return isinstance(getattr(module, "gate", None), nn.Linear) and hasattr(module, "experts") and len(module.experts) > 0
+
+
+def make_sparseflow_moe(module: nn.Module, top_k: Optional[int] = None, renormalize: Optional[bool] = None) -> SparseFlowMoE:
+    """From a module with a router ``gate`` (``nn.Linear``) and a list ``experts`` of gated MLPs (``gate_proj / up_proj / down_proj`` or
+    ``w1 / w3 / w2``).  ``top_k`` and ``renormalize`` default to the module's ``top_k`` and ``norm_topk_prob`` (True without one)."""
+    from .surgery import _get_mlp_projections
+    if not is_moe(module):
+        raise RuntimeError(f"Unsupported MoE layout: {type(module)}")
+    if top_k is None:
+        top_k = getattr(module, "top_k", None)
+        if top_k is None:
+            raise ValueError("top_k is not given and the module has none")
+    if renormalize is None:
+        renormalize = bool(getattr(module, "norm_topk_prob", True))
+    gates, ups, downs = zip(*(_get_mlp_projections(e) for e in module.experts))
+    (g, gb), (u, ub), (d, db) = _stacked(gates, "gate"), _stacked(ups, "up"), _stacked(downs, "down")
+    router = module.gate
+    return SparseFlowMoE(router.weight, g, u, d, top_k, renormalize, gb, ub, db, router.bias)

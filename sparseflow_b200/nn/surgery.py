@@ -4,6 +4,7 @@ Interface of the reference's ``sparseflow/nn/surgery.py:22-99`` (``replace_llama
 policy, verbose)`` -> number of layers replaced): walks ``model.model.layers`` or ``model.layers``,
 accepts the ``gate_proj/up_proj/down_proj`` and ``w1/w3/w2`` layouts, and builds the replacement from
 the layer's own weights.  ``down_mode`` is passed through (default "dense", the reference's function).
+A mixture of experts (a router ``gate`` and a list ``experts`` of such MLPs) becomes a ``SparseFlowMoE``, whose products are all sparse.
 """
 from __future__ import annotations
 
@@ -11,6 +12,7 @@ import torch
 import torch.nn as nn
 
 from .sparseflow_mlp import SparseFlowMLP
+from .sparseflow_moe import is_moe, make_sparseflow_moe
 
 
 def _get_mlp_projections(mlp: nn.Module):
@@ -33,6 +35,13 @@ def replace_llama_mlp_module(model: nn.Module, policy, verbose: bool = False, do
     replaced = 0
     for i, layer in enumerate(_layers_of(model)):
         if not hasattr(layer, "mlp"):
+            continue
+        if is_moe(layer.mlp):
+            with torch.inference_mode(False):
+                layer.mlp = make_sparseflow_moe(layer.mlp)
+            replaced += 1
+            if verbose:
+                print(f"  layer {i:02d} mlp -> SparseFlowMoE")
             continue
         gate, up, down = _get_mlp_projections(layer.mlp)
         bias = lambda m: None if getattr(m, "bias", None) is None else m.bias.detach()

@@ -8,7 +8,10 @@ model hub; here the stack is built from its SHAPE with seeded random weights and
 follows the usual decoder layout (``model.layers[i].self_attn.{q,k,v,o}_proj``,
 ``model.layers[i].mlp.{gate,up,down}_proj``) so ``replace_llama_mlp_module`` applies unchanged.
 
-    python -m sparseflow_b200.prefill_e2e --layers 4 --batch 2 --seq 2048 [--json out.json]
+A last arm runs the norms fused with the sums in front of them (``SparseFlowBlockNorm``).  With ``--experts`` every MLP is a mixture of
+experts, which the surgery turns into ``SparseFlowMoE``.
+
+    python -m sparseflow_b200.prefill_e2e --layers 4 --batch 2 --seq 2048 [--experts 8 --top-k 2] [--json out.json]
 """
 from __future__ import annotations
 
@@ -20,7 +23,7 @@ import torch
 import torch.nn as nn
 import torch.nn.functional as F
 
-from .nn import SparseFlowPolicy, prune_24_dense_weight, replace_llama_mlp_module
+from .nn import SparseFlowBlockNorm, SparseFlowPolicy, prune_24_dense_weight, replace_llama_mlp_module
 
 
 class RMSNorm(nn.Module):
@@ -65,13 +68,34 @@ class GatedMLP(nn.Module):
         return self.down_proj(F.silu(self.gate_proj(x)) * self.up_proj(x))
 
 
+class MoEMLP(nn.Module):
+    """A router and a list of gated MLPs, each run on its own tokens: the layout ``make_sparseflow_moe`` reads."""
+
+    def __init__(self, hidden, inter, experts, top_k, **kw):
+        super().__init__()
+        self.gate = nn.Linear(hidden, experts, bias=False, **kw)
+        self.experts = nn.ModuleList([GatedMLP(hidden, inter, **kw) for _ in range(experts)])
+        self.top_k = top_k
+
+    def forward(self, x):
+        x2d = x.reshape(-1, x.shape[-1])
+        value, index = torch.topk(self.gate(x2d).float(), self.top_k, dim=-1)
+        weight = torch.softmax(value, -1)
+        out = torch.zeros_like(x2d, dtype=torch.float32)
+        for e, expert in enumerate(self.experts):
+            token, slot = (index == e).nonzero(as_tuple=True)
+            if token.numel():
+                out.index_add_(0, token, expert(x2d[token]).float() * weight[token, slot, None])
+        return out.to(x.dtype).view_as(x)
+
+
 class DecoderLayer(nn.Module):
-    def __init__(self, hidden, inter, heads, **kw):
+    def __init__(self, hidden, inter, heads, experts=0, top_k=2, **kw):
         super().__init__()
         self.input_layernorm = RMSNorm(hidden, **kw)
         self.self_attn = Attention(hidden, heads, **kw)
         self.post_attention_layernorm = RMSNorm(hidden, **kw)
-        self.mlp = GatedMLP(hidden, inter, **kw)
+        self.mlp = MoEMLP(hidden, inter, experts, top_k, **kw) if experts else GatedMLP(hidden, inter, **kw)
 
     def forward(self, x, rope):
         x = x + self.self_attn(self.input_layernorm(x), rope)
@@ -81,14 +105,15 @@ class DecoderLayer(nn.Module):
 class LlamaShapedStack(nn.Module):
     """Embedding -> N decoder layers -> norm.  (No LM head: prefill cost is the layers'.)"""
 
-    def __init__(self, layers, hidden, inter, heads, vocab=32000, device="cuda", dtype=torch.bfloat16, seed=0):
+    def __init__(self, layers, hidden, inter, heads, vocab=32000, device="cuda", dtype=torch.bfloat16, seed=0, experts=0, top_k=2):
         super().__init__()
         kw = dict(device=device, dtype=dtype)
         torch.manual_seed(seed)
         self.embed_tokens = nn.Embedding(vocab, hidden, **kw)
-        self.layers = nn.ModuleList([DecoderLayer(hidden, inter, heads, **kw) for _ in range(layers)])
+        self.layers = nn.ModuleList([DecoderLayer(hidden, inter, heads, experts, top_k, **kw) for _ in range(layers)])
         self.norm = RMSNorm(hidden, **kw)
         self.head_dim = hidden // heads
+        self.fused_norms = None      # [SparseFlowBlockNorm] in the order of the norms, by fuse_norms
         for p in self.parameters():
             if p.dim() == 2:
                 p.data.normal_(0, 0.02)
@@ -103,9 +128,22 @@ class LlamaShapedStack(nn.Module):
     def forward(self, ids):
         x = self.embed_tokens(ids)
         rope = self.rope(ids.shape[1], ids.device, x.dtype)
+        if self.fused_norms is not None:
+            norms = iter(self.fused_norms)
+            x, h = next(norms)(x)
+            for layer in self.layers:
+                x, h = next(norms)(x, layer.self_attn(h, rope))
+                x, h = next(norms)(x, layer.mlp(h))
+            return h
         for layer in self.layers:
             x = layer(x, rope)
         return self.norm(x)
+
+    def fuse_norms(self):
+        """Every norm together with the sum in front of it, one kernel each."""
+        chain = [n for layer in self.layers for n in (layer.input_layernorm, layer.post_attention_layernorm)] + [self.norm]
+        self.fused_norms = [SparseFlowBlockNorm(n.weight, eps=n.eps) for n in chain]
+        return len(chain)
 
 
 class _MlpTimer:
@@ -163,22 +201,23 @@ def sparsify_attention(model, policy) -> int:
 
 
 def run(layers=4, hidden=4096, inter=11008, heads=32, batch=2, seq=2048, dtype="bf16", iters=10, warmup=3,
-        attention=True) -> dict:
+        attention=True, experts=0, top_k=2) -> dict:
     td = torch.bfloat16 if dtype == "bf16" else torch.float16
-    model = LlamaShapedStack(layers, hidden, inter, heads, dtype=td).eval()
+    model = LlamaShapedStack(layers, hidden, inter, heads, dtype=td, experts=experts, top_k=top_k).eval()
     g = torch.Generator(device="cpu").manual_seed(1234)
     ids = torch.randint(0, 32000, (batch, seq), generator=g).cuda()
     res = {"config": dict(layers=layers, hidden=hidden, inter=inter, heads=heads, batch=batch, seq=seq,
                           tokens=batch * seq, dtype=dtype, weights="seeded random N(0, 0.02), no checkpoint",
-                          iters=iters, warmup=warmup), "arms": {}}
+                          iters=iters, warmup=warmup, experts=experts, top_k=top_k if experts else None), "arms": {}}
 
     def arm(name):
         ms, mlp_ms = time_arm(model, ids, iters, warmup)
         res["arms"][name] = dict(ms=ms, mlp_ms=mlp_ms, mlp_share=mlp_ms / ms, tokens_per_s=batch * seq / ms * 1e3)
 
     arm("dense")
+    routers = [m.gate for m in model.modules() if isinstance(m, MoEMLP)]
     for m in model.modules():                       # every Linear, as the reference's pruned-dense arm does
-        if isinstance(m, nn.Linear):
+        if isinstance(m, nn.Linear) and m not in routers:
             m.weight.data.copy_(prune_24_dense_weight(m.weight.data))
     ref_out = model(ids)
     arm("pruned_dense")
@@ -194,6 +233,11 @@ def run(layers=4, hidden=4096, inter=11008, heads=32, batch=2, seq=2048, dtype="
         res["attn_linears_replaced"] = sparsify_attention(model, policy)
         res["attn_uses_sparse_at_this_M"] = policy.should_use_sparse("q_proj", M)
         arm("sparse_mlp_attn")
+    before = model(ids)
+    res["norms_fused"] = model.fuse_norms()
+    after = model(ids)
+    res["fused_norms_max_err_over_max"] = (after.float() - before.float()).abs().max().item() / before.float().abs().max().item()
+    arm("fused_norms")
     a = res["arms"]
     res["speedup_sparse_vs_pruned_dense"] = a["pruned_dense"]["ms"] / a["sparse_mlp"]["ms"]
     res["speedup_sparse_vs_dense"] = a["dense"]["ms"] / a["sparse_mlp"]["ms"]
@@ -213,10 +257,13 @@ def main():
     ap.add_argument("--iters", type=int, default=10)
     ap.add_argument("--warmup", type=int, default=3)
     ap.add_argument("--no-attention", action="store_true")
+    ap.add_argument("--experts", type=int, default=0, help="experts per MLP (0: one gated MLP)")
+    ap.add_argument("--top-k", type=int, default=2, help="experts per token")
     ap.add_argument("--json", default=None)
     a = ap.parse_args()
     assert torch.cuda.is_available(), "CUDA required"
-    r = run(a.layers, a.hidden, a.inter, a.heads, a.batch, a.seq, a.dtype, a.iters, a.warmup, not a.no_attention)
+    r = run(a.layers, a.hidden, a.inter, a.heads, a.batch, a.seq, a.dtype, a.iters, a.warmup, not a.no_attention,
+            a.experts, a.top_k)
     for name, v in r["arms"].items():
         print(f"{name:16s} {v['ms']:8.3f} ms   MLP {v['mlp_ms']:8.3f} ms ({100 * v['mlp_share']:.1f} %)   "
               f"{v['tokens_per_s']:.0f} tok/s")
