@@ -17,7 +17,6 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
-#include <math.h>
 #include <stdint.h>
 
 #include "grouped.cuh"
@@ -271,26 +270,31 @@ __global__ void __launch_bounds__(256) gather_rows_kernel(const uint16_t* src, i
 }
 
 // Estimated time in us of a variant (32, 64: single-CTA tiles of that many tokens; 1128, 1240, 2128, 2240: pair tiles of 256 or 512
-// rows) with all experts of the average size: passes over the SMs or pairs x (128-wide K steps x step time + drain), and the weights at
-// 6.2 TB/s; the shorter of the two adds a sixth.  Constants fitted to 450 runs on 13 weight sets (1000-22016 rows, K 512-11008, 4-128
-// experts, 4-1024 tokens per expert with ragged sizes; relative error 0.1); the choice by it averages 1.02 of the fastest variant.
+// rows) from the average tokens per expert: launch + passes over the SMs or pairs x (128-wide K steps x step time + drain), or the weights at
+// 6.2 TB/s, and a sixth of the shorter of the two.  Sizes are ragged: an expert takes half a tile more than its tokens fill, once they fill
+// three quarters of one.  Constants fitted to 200 settings under steady load, every variant timed on each (1000-22016 rows, K 512-11008, 4-128 experts,
+// 1-1000 tokens per expert; relative error 0.1).  The choice by it averages 1.02 of the fastest variant (gathered rows: 1.03), worst 1.27.
 double grouped_cost(int variant, bool gather, int total, int experts, int n_out, int K, int num_sms) {
-  struct Step { int rows, tokens, variant; double base, per_token, drain, tail, g_base, g_per_token, g_drain, g_tail; };
-  static const Step steps[] = {
-      {128, 32, 32, 0.0255, 0.0038, 1.6, 1.0, 0.054, 0.0082, 1.8, 0.65},    {128, 64, 64, 0.131, 0.0011, 1.3, 0.77, 0.138, 0.0051, 1.7, 0.47},
-      {256, 128, 1128, 0.182, 0.0005, 1.7, 0.65, 0.40, 0.0020, 3.0, 0.4},   {256, 240, 1240, 0.257, 0.0005, 1.8, 0.65, 0.243, 0.0014, 1.9, 0.40},
-      {512, 128, 2128, 0.281, 0.0011, 3.6, 0.74, 0.261, 0.0023, 3.4, 0.56}, {512, 240, 2240, 0.323, 0.0016, 4.5, 0.67, 0.308, 0.0024, 4.4, 0.57}};
-  for (const Step& s : steps) {
-    if (s.variant != variant) continue;
+  struct Step { double base, per_token, drain, tail, launch; };
+  struct Form { int variant, rows, tokens; Step plain, gather; };
+  static const Form forms[] = {
+      {32, 128, 32, {0.0, 0.008, 0.21, 0.02, 3.6}, {0.248, 0.0044, 0.52, 0.80, 0.0}},
+      {64, 128, 64, {0.2325, 0.0005, 0.58, 0.20, 1.6}, {0.218, 0.0066, 0.58, 0.0, 0.0}},
+      {1128, 256, 128, {0.219, 0.0005, 1.35, 0.92, 2.6}, {0.0, 0.0045, 0.62, 0.0, 5.3}},
+      {1240, 256, 240, {0.265, 0.0009, 1.46, 0.93, 3.5}, {0.315, 0.0015, 1.35, 0.47, 0.0}},
+      {2128, 512, 128, {0.329, 0.0015, 3.87, 0.97, 0.0}, {0.3325, 0.0018, 2.98, 0.89, 1.1}},
+      {2240, 512, 240, {0.359, 0.0026, 4.08, 0.78, 0.0}, {0.375, 0.0028, 3.86, 0.72, 0.0}}};
+  for (const Form& f : forms) {
+    if (f.variant != variant) continue;
+    const Step& s = gather ? f.gather : f.plain;
     const double avg = total > experts ? static_cast<double>(total) / experts : 1.0;
     const double active = total < experts ? total : experts;
-    const int cuts = static_cast<int>(ceil(avg / s.tokens));
-    const double tiles = active * ((n_out + s.rows - 1) / s.rows) * cuts, units = s.rows == 128 ? num_sms : num_sms / 2;
-    const double passes = tiles > units ? tiles / units + (gather ? s.g_tail : s.tail) : 1.0;
-    const double step = (gather ? s.g_base : s.base) + (gather ? s.g_per_token : s.per_token) * (avg / cuts);
-    const double work = passes * (((K + 127) / 128) * step + (gather ? s.g_drain : s.drain));
+    const double cuts = avg <= 0.75 * f.tokens ? 1.0 : avg / f.tokens + 0.5;
+    const double tiles = active * ((n_out + f.rows - 1) / f.rows) * cuts, units = f.rows == 128 ? num_sms : num_sms / 2;
+    const double passes = tiles > units ? tiles / units + s.tail : 1.0;
+    const double work = passes * (((K + 127) / 128) * (s.base + s.per_token * (avg / cuts)) + s.drain);
     const double hbm = active * n_out * (K * 1.125) / 6.2e6;
-    return 5.0 + (work > hbm ? work + 0.15 * hbm : hbm + 0.15 * work);
+    return s.launch + (work > hbm ? work + 0.15 * hbm : hbm + 0.15 * work);
   }
   return 1e30;
 }
@@ -309,7 +313,7 @@ int plan_grouped(int total, int experts, int n_out, int K, bool gather, int num_
     if (c < cost) { cost = c; best = v; }
   }
   if (!gather) return best;
-  const double copy = 2.5 + static_cast<double>(total) * K * 4.0 / 5.5e6;
+  const double copy = 3.0 + static_cast<double>(total) * K * 4.0 / 7.4e6;
   for (int v : variants) {
     const double c = copy + grouped_cost(v, false, total, experts, n_out, K, num_sms);
     if (c < cost) { cost = c; best = 10000 + v; }
