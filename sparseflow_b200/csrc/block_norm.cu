@@ -12,12 +12,15 @@
 // the columns of a whole piece, 8j - m .. with m the row's offset, reads it with the neighbour's values in it (inside the tensor) and drops those; the
 // pieces at the ends of a row are stored value by value, and weights, which begin at column 0, are shifted by m from two pieces.
 // Value by value throughout where the tensors' rows do not lie alike in their pieces.
-//   4096 x 8192 (f32 stream, bf16, norm on both sides) 83 us (4.8 TB/s), 16384 x 2048 bf16 58 us, 24 x 4096 2.8 us (latency).
+// Measured: 4096 x 8192 (f32 stream, bf16, norm on both sides) 78 us (5.2 TB/s), 16384 x 2048 bf16 58 us (4.6 TB/s; issue-bound: 50 instructions
+// a piece), 8192 x 4097 layer norms 122 us, 24 x 4096 2.8 us (latency).
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 #include <stdint.h>
 #include <string.h>
+
+#include <atomic>
 
 #include "kernels.h"
 #include "launch.h"
@@ -149,172 +152,283 @@ __device__ __forceinline__ void load_vector(const void* base, int64_t first, int
   }
 }
 
+// Asynchronous copy of `bytes` (0 .. 16, the rest zero) to shared memory
+__device__ __forceinline__ void copy16(uint32_t dst, const void* src, int bytes) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+template <class T, int V>
+__device__ __forceinline__ void copy_piece(uint32_t dst, const void* base, int64_t at, int64_t room) {
+  const T* src = static_cast<const T*>(base) + at;
+#pragma unroll
+  for (int b = 0; b < V * static_cast<int>(sizeof(T)); b += 16) {
+    const int64_t left = room * static_cast<int64_t>(sizeof(T)) - b;
+    const int bytes = left >= 16 ? 16 : left > 0 ? static_cast<int>(left) : 0;
+    copy16(dst + b, bytes > 0 ? reinterpret_cast<const uint8_t*>(src) + b : base, bytes);
+  }
+}
+
 // XT: type of x and r; YT: type of y, h, weights and gate.  WARP: a warp per row, eight rows per block; otherwise a block per row.
-template <class XT, class YT, int V, int NV, bool SHIFT, bool LAYER, bool WARP, int MAXT, int MINB>
+// RING: blocks stay; while a row is reduced, asynchronous copies bring the next one into shared memory, every thread its own pieces, so
+// that nobody waits for anybody.  With SHIFT the block's rows are eight apart or a multiple of it: one m, and the vectors are shifted once, into
+// shared memory too (`vectors` of them, in the order post_bias, post_weight, weight, bias, gate where all rows share it).
+template <class XT, class YT, int V, int NV, bool SHIFT, bool LAYER, bool WARP, bool RING, int MAXT, int MINB>
 __global__ void __launch_bounds__(MAXT, MINB) block_norm_kernel(const NormParams p) {
   __shared__ __align__(16) float part[2][32];
+  extern __shared__ __align__(16) uint8_t ring[];
   dependency_wait();
   dependency_trigger();
-  const int row_i = WARP ? static_cast<int>(blockIdx.x * 8 + (threadIdx.x >> 5)) : static_cast<int>(blockIdx.x);
-  if (WARP && row_i >= p.rows) return;
-  const int64_t row = row_i;
-  const int m = SHIFT ? static_cast<int>(row * p.ld_x & 7) : 0;
+  int row_i = WARP ? static_cast<int>(blockIdx.x * 8 + (threadIdx.x >> 5)) : static_cast<int>(blockIdx.x);
+  if (row_i >= p.rows) return;
+  const int m = SHIFT ? static_cast<int>(row_i * p.ld_x & 7) : 0;
   const int c0 = static_cast<int>(WARP ? threadIdx.x & 31 : threadIdx.x) * V - m, step = (WARP ? 32 : static_cast<int>(blockDim.x)) * V;
   auto outside = [&](int c, int i) { return c + i < 0 || c + i >= p.cols; };
   int turn = 0;
-  Pack<XT, V> xv[NV];
-  Pack<YT, V> yv[NV];
+  Pack<XT, V>* x_slot = reinterpret_cast<Pack<XT, V>*>(ring) + threadIdx.x;                          // [NV][threads]
+  Pack<YT, V>* y_slot = reinterpret_cast<Pack<YT, V>*>(ring + NV * blockDim.x * sizeof(Pack<XT, V>)) + threadIdx.x;
+  Pack<YT, V>* vectors = y_slot + NV * blockDim.x;                                                   // [vector][NV][threads]
+  auto fetch = [&](int r) {
+    const int64_t row = r, behind = p.rows - 1 - row;
+    if (r < p.rows) {
 #pragma unroll
-  for (int n = 0; n < NV; ++n) {
-    const int c = c0 + n * step;
-    if (c < p.cols) {
-      const int64_t behind = p.rows - 1 - row;
-      xv[n] = load_piece<XT, V, SHIFT>(p.x, row * p.ld_x + c, behind * p.ld_x + p.cols - c);
-      if (p.y != nullptr) yv[n] = load_piece<YT, V, SHIFT>(p.y, row * p.ld_y + c, behind * p.ld_y + p.cols - c);
-    } else {
-#pragma unroll
-      for (int i = 0; i < V; ++i) {
-        xv[n].v[i] = from_f<XT>(0.f);
-        yv[n].v[i] = from_f<YT>(0.f);
+      for (int n = 0; n < NV; ++n) {
+        const int c = c0 + n * step;
+        if (c >= p.cols) continue;
+        copy_piece<XT, V>(smem_u32(x_slot + n * blockDim.x), p.x, row * p.ld_x + c, behind * p.ld_x + p.cols - c);
+        if (p.y != nullptr) copy_piece<YT, V>(smem_u32(y_slot + n * blockDim.x), p.y, row * p.ld_y + c, behind * p.ld_y + p.cols - c);
       }
     }
-    if (SHIFT && (c < 0 || c + V > p.cols)) {
+  };
+  const bool one_gate = p.gate != nullptr && p.gate_step != 0 && p.rows_per_gate >= p.rows;
+  auto vector = [&](const void* base, int64_t first, int which, int n, int c, bool pieces, float* f) {
+    if (RING && SHIFT && which >= 0) {
+      const Pack<YT, V> k = vectors[(which * NV + n) * blockDim.x];
 #pragma unroll
-      for (int i = 0; i < V; ++i)
-        if (outside(c, i)) {
-          xv[n].v[i] = from_f<XT>(0.f);
-          yv[n].v[i] = from_f<YT>(0.f);
-        }
+      for (int i = 0; i < V; ++i) f[i] = to_f<YT>(k.v[i]);
+    } else {
+      load_vector<YT, V, SHIFT>(base, first, c, p.cols, m, pieces, f);
+    }
+  };
+  if (RING) {
+    fetch(row_i);
+    if (SHIFT) {
+      const void* all[5] = {p.post_bias, p.post_weight, p.weight, p.bias, one_gate ? p.gate : nullptr};
+#pragma unroll
+      for (int k = 0; k < 5; ++k)
+        if (all[k] != nullptr)
+#pragma unroll
+          for (int n = 0; n < NV; ++n) {
+            float f[V];
+            load_vector<YT, V, SHIFT>(all[k], 0, c0 + n * step, p.cols, m, true, f);
+            Pack<YT, V> v;
+#pragma unroll
+            for (int i = 0; i < V; ++i) v.v[i] = from_f<YT>(f[i]);      // as they were: the type's own values
+            vectors[(k * NV + n) * blockDim.x] = v;
+          }
     }
   }
-  // 1 / sqrt(mean of squares + eps) of values that are zero outside the row; layer: of the centered values, `mean` theirs
-  auto inverse_norm = [&](auto value, float eps, float& mean) {
-    float s = 0.f;
-    if (LAYER) {
-#pragma unroll
-      for (int n = 0; n < NV; ++n)
-#pragma unroll
-        for (int i = 0; i < V; ++i) s += value(n, i);
-      mean = row_sum<WARP>(s, part, turn) * p.inv_cols;
-      s = 0.f;
-    }
-#pragma unroll
-    for (int n = 0; n < NV; ++n) {
-      const int c = c0 + n * step;
-#pragma unroll
-      for (int i = 0; i < V; ++i) {
-        float d = value(n, i);
-        if (LAYER) d = (SHIFT ? outside(c, i) : c >= p.cols) ? 0.f : d - mean;
-        s = fmaf(d, d, s);
-      }
-    }
-    return rsqrtf(row_sum<WARP>(s, part, turn) * p.inv_cols + eps);
-  };
-  float f[NV][V];
-  if (p.y != nullptr) {
-    float z_mean = 0.f, z_inv = 1.f;
-    if (p.post_weight != nullptr) z_inv = inverse_norm([&](int n, int i) { return to_f<YT>(yv[n].v[i]); }, p.post_eps, z_mean);
-    const int64_t gate_row = p.gate != nullptr ? static_cast<int64_t>(row_i / p.rows_per_gate) * p.ld_gate : 0;
-    const bool per_col = p.gate != nullptr && p.gate_step != 0;
-    const float row_gate = p.scale * (p.gate != nullptr && !per_col ? to_f<YT>(static_cast<const YT*>(p.gate)[gate_row]) : 1.f);
+  for (;;) {
+    const int64_t row = row_i;
+    bool fetched = !RING;
+    // the next row may replace this one in shared memory once it is in registers: behind the first sum over the row
+    auto fetch_next = [&]() {
+      if (!fetched) fetch(row_i + static_cast<int>(gridDim.x));
+      fetched = true;
+    };
+    Pack<XT, V> xv[NV];
+    Pack<YT, V> yv[NV];
+    if (RING) asm volatile("cp.async.wait_all;" ::: "memory");
 #pragma unroll
     for (int n = 0; n < NV; ++n) {
       const int c = c0 + n * step;
       if (c < p.cols) {
-        // f = x + factor * (z - mean) + offset: factor = scale * gate * inverse norm * post weight, offset = scale * gate * post bias
-        float factor[V], w[V];
-#pragma unroll
-        for (int i = 0; i < V; ++i) f[n][i] = to_f<XT>(xv[n].v[i]);
-        if (per_col) {
-          load_vector<YT, V, SHIFT>(p.gate, gate_row, c, p.cols, m, gate_row % 8 == 0, factor);
-          if (p.post_bias != nullptr) {
-            load_vector<YT, V, SHIFT>(p.post_bias, 0, c, p.cols, m, true, w);
-#pragma unroll
-            for (int i = 0; i < V; ++i) f[n][i] = fmaf(p.scale * factor[i], w[i], f[n][i]);
-          }
-          if (p.post_weight != nullptr) {
-            load_vector<YT, V, SHIFT>(p.post_weight, 0, c, p.cols, m, true, w);
-#pragma unroll
-            for (int i = 0; i < V; ++i) factor[i] *= w[i];
-          }
-        } else {
-          if (p.post_bias != nullptr) {
-            load_vector<YT, V, SHIFT>(p.post_bias, 0, c, p.cols, m, true, w);
-#pragma unroll
-            for (int i = 0; i < V; ++i) f[n][i] = fmaf(row_gate, w[i], f[n][i]);
-          }
-          if (p.post_weight != nullptr) {
-            load_vector<YT, V, SHIFT>(p.post_weight, 0, c, p.cols, m, true, factor);
-          } else {
-#pragma unroll
-            for (int i = 0; i < V; ++i) factor[i] = 1.f;
-          }
-        }
-        const float common = (per_col ? p.scale : row_gate) * z_inv;
-#pragma unroll
-        for (int i = 0; i < V; ++i) {
-          const float z = to_f<YT>(yv[n].v[i]);
-          f[n][i] = fmaf((LAYER ? z - z_mean : z) * common, factor[i], f[n][i]);
-        }
-        store_piece<XT, V, SHIFT>(p.r, row * p.ld_r + c, c, p.cols, f[n]);
-        if (SHIFT && (c < 0 || c + V > p.cols)) {
-#pragma unroll
-          for (int i = 0; i < V; ++i)
-            if (outside(c, i)) f[n][i] = 0.f;
-        }
+        const int64_t behind = p.rows - 1 - row;
+        xv[n] = RING ? x_slot[n * blockDim.x] : load_piece<XT, V, SHIFT>(p.x, row * p.ld_x + c, behind * p.ld_x + p.cols - c);
+        if (p.y != nullptr) yv[n] = RING ? y_slot[n * blockDim.x] : load_piece<YT, V, SHIFT>(p.y, row * p.ld_y + c, behind * p.ld_y + p.cols - c);
       } else {
 #pragma unroll
-        for (int i = 0; i < V; ++i) f[n][i] = 0.f;
+        for (int i = 0; i < V; ++i) {
+          xv[n].v[i] = from_f<XT>(0.f);
+          yv[n].v[i] = from_f<YT>(0.f);
+        }
+      }
+      if (SHIFT && (c < 0 || c + V > p.cols)) {
+#pragma unroll
+        for (int i = 0; i < V; ++i)
+          if (outside(c, i)) {
+            xv[n].v[i] = from_f<XT>(0.f);
+            yv[n].v[i] = from_f<YT>(0.f);
+          }
       }
     }
-  } else {
+    // 1 / sqrt(mean of squares + eps) of values that are zero outside the row; layer: of the centered values, `mean` theirs
+    auto inverse_norm = [&](auto value, float eps, float& mean) {
+      float s = 0.f;
+      if (LAYER) {
 #pragma unroll
-    for (int n = 0; n < NV; ++n)
+        for (int n = 0; n < NV; ++n)
 #pragma unroll
-      for (int i = 0; i < V; ++i) f[n][i] = to_f<XT>(xv[n].v[i]);
-  }
-  if (p.h == nullptr) return;
-  float mean = 0.f;
-  const float inv = inverse_norm([&](int n, int i) { return f[n][i]; }, p.eps, mean);
-#pragma unroll
-  for (int n = 0; n < NV; ++n) {
-    const int c = c0 + n * step;
-    if (c < p.cols) {
-      float w[V];
-      load_vector<YT, V, SHIFT>(p.weight, 0, c, p.cols, m, true, w);
-#pragma unroll
-      for (int i = 0; i < V; ++i) f[n][i] = ((LAYER ? f[n][i] - mean : f[n][i]) * inv) * w[i];
-      if (p.bias != nullptr) {
-        load_vector<YT, V, SHIFT>(p.bias, 0, c, p.cols, m, true, w);
-#pragma unroll
-        for (int i = 0; i < V; ++i) f[n][i] += w[i];
+          for (int i = 0; i < V; ++i) s += value(n, i);
+        mean = row_sum<WARP>(s, part, turn) * p.inv_cols;
+        fetch_next();
+        s = 0.f;
       }
-      store_piece<YT, V, SHIFT>(p.h, row * p.ld_h + c, c, p.cols, f[n]);
+#pragma unroll
+      for (int n = 0; n < NV; ++n) {
+        const int c = c0 + n * step;
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+          float d = value(n, i);
+          if (LAYER) d = (SHIFT ? outside(c, i) : c >= p.cols) ? 0.f : d - mean;
+          s = fmaf(d, d, s);
+        }
+      }
+      s = row_sum<WARP>(s, part, turn);
+      fetch_next();
+      return rsqrtf(s * p.inv_cols + eps);
+    };
+    float f[NV][V];
+    if (p.y != nullptr) {
+      float z_mean = 0.f, z_inv = 1.f;
+      if (p.post_weight != nullptr) z_inv = inverse_norm([&](int n, int i) { return to_f<YT>(yv[n].v[i]); }, p.post_eps, z_mean);
+      const int64_t gate_row = p.gate != nullptr ? static_cast<int64_t>(row_i / p.rows_per_gate) * p.ld_gate : 0;
+      const bool per_col = p.gate != nullptr && p.gate_step != 0;
+      const float row_gate = p.scale * (p.gate != nullptr && !per_col ? to_f<YT>(static_cast<const YT*>(p.gate)[gate_row]) : 1.f);
+#pragma unroll
+      for (int n = 0; n < NV; ++n) {
+        const int c = c0 + n * step;
+        if (c < p.cols) {
+          // f = x + factor * (z - mean) + offset: factor = scale * gate * inverse norm * post weight, offset = scale * gate * post bias
+          float factor[V], w[V];
+#pragma unroll
+          for (int i = 0; i < V; ++i) f[n][i] = to_f<XT>(xv[n].v[i]);
+          if (per_col) {
+            vector(p.gate, gate_row, one_gate ? 4 : -1, n, c, gate_row % 8 == 0, factor);
+            if (p.post_bias != nullptr) {
+              vector(p.post_bias, 0, 0, n, c, true, w);
+#pragma unroll
+              for (int i = 0; i < V; ++i) f[n][i] = fmaf(p.scale * factor[i], w[i], f[n][i]);
+            }
+            if (p.post_weight != nullptr) {
+              vector(p.post_weight, 0, 1, n, c, true, w);
+#pragma unroll
+              for (int i = 0; i < V; ++i) factor[i] *= w[i];
+            }
+          } else {
+            if (p.post_bias != nullptr) {
+              vector(p.post_bias, 0, 0, n, c, true, w);
+#pragma unroll
+              for (int i = 0; i < V; ++i) f[n][i] = fmaf(row_gate, w[i], f[n][i]);
+            }
+            if (p.post_weight != nullptr) {
+              vector(p.post_weight, 0, 1, n, c, true, factor);
+            } else {
+#pragma unroll
+              for (int i = 0; i < V; ++i) factor[i] = 1.f;
+            }
+          }
+          const float common = (per_col ? p.scale : row_gate) * z_inv;
+#pragma unroll
+          for (int i = 0; i < V; ++i) {
+            const float z = to_f<YT>(yv[n].v[i]);
+            f[n][i] = fmaf((LAYER ? z - z_mean : z) * common, factor[i], f[n][i]);
+          }
+          store_piece<XT, V, SHIFT>(p.r, row * p.ld_r + c, c, p.cols, f[n]);
+          if (SHIFT && (c < 0 || c + V > p.cols)) {
+#pragma unroll
+            for (int i = 0; i < V; ++i)
+              if (outside(c, i)) f[n][i] = 0.f;
+          }
+        } else {
+#pragma unroll
+          for (int i = 0; i < V; ++i) f[n][i] = 0.f;
+        }
+      }
+    } else {
+#pragma unroll
+      for (int n = 0; n < NV; ++n)
+#pragma unroll
+        for (int i = 0; i < V; ++i) f[n][i] = to_f<XT>(xv[n].v[i]);
     }
+    if (p.h != nullptr) {
+      float mean = 0.f;
+      const float inv = inverse_norm([&](int n, int i) { return f[n][i]; }, p.eps, mean);
+#pragma unroll
+      for (int n = 0; n < NV; ++n) {
+        const int c = c0 + n * step;
+        if (c < p.cols) {
+          float w[V];
+          vector(p.weight, 0, 2, n, c, true, w);
+#pragma unroll
+          for (int i = 0; i < V; ++i) f[n][i] = ((LAYER ? f[n][i] - mean : f[n][i]) * inv) * w[i];
+          if (p.bias != nullptr) {
+            vector(p.bias, 0, 3, n, c, true, w);
+#pragma unroll
+            for (int i = 0; i < V; ++i) f[n][i] += w[i];
+          }
+          store_piece<YT, V, SHIFT>(p.h, row * p.ld_h + c, c, p.cols, f[n]);
+        }
+      }
+    } else if (RING) {
+      __syncthreads();
+      fetch_next();
+    }
+    if (!RING) break;
+    row_i += static_cast<int>(gridDim.x);
+    if (row_i >= p.rows) break;
   }
 }
 
+// Rows and pieces of a row from which blocks stay: with a row or two each there is nothing to fetch ahead, and eight or more short rows per SM cover each
+// other (16384 x 1024 f32 38 us, with the ring 44; 3000 x 1001 8.6 and 10.6; 4096 x 8192 f32 83 and 78, 8192 x 4097 layer norms 160 and 122).
+constexpr int kRingRows = 4 * 148, kRingPieces = 257;
+
+template <class Kernel>
+int launch_ring(Kernel kernel, const NormParams& p, int threads, int smem, bool shift, int num_sms, std::atomic<int>* known, cudaStream_t stream) {
+  // blocks per SM, asked for once per block size and shared-memory size (both change rarely)
+  std::atomic<int>& slot = known[threads / 32];
+  int per_sm = slot.load(std::memory_order_relaxed);
+  if (per_sm / 16 != smem / 16) {
+    int n = 0;
+    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 220 * 1024) != cudaSuccess ||
+        cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kernel, threads, smem) != cudaSuccess || n < 1)
+      return kErrCuda;
+    per_sm = smem / 16 * 16 + (n < 15 ? n : 15);
+    slot.store(per_sm, std::memory_order_relaxed);
+  }
+  int grid = num_sms * (per_sm % 16);
+  if (shift) grid = grid / 8 * 8;      // one m per block
+  return launch_dependent(kernel, grid < p.rows ? grid : p.rows, threads, smem, 0, stream, p);
+}
+
 template <class XT, class YT, bool SHIFT, bool LAYER>
-int launch_pieces(const NormParams& p, cudaStream_t stream) {
+int launch_pieces(const NormParams& p, int num_sms, cudaStream_t stream) {
   const int pieces = (p.cols + (SHIFT ? 14 : 7)) / 8;      // a row may begin at the last value of a piece
   auto threads = [&](int nv) { return ((pieces + nv - 1) / nv + 31) / 32 * 32; };
   const int groups = (p.rows + 7) / 8;
-  if (pieces <= 32) return launch_dependent(block_norm_kernel<XT, YT, 8, 1, SHIFT, LAYER, true, 256, 5>, groups, 256, 0, 0, stream, p);
-  if (pieces <= 64) return launch_dependent(block_norm_kernel<XT, YT, 8, 2, SHIFT, LAYER, true, 256, 4>, groups, 256, 0, 0, stream, p);
-  if (pieces <= 512) return launch_dependent(block_norm_kernel<XT, YT, 8, 2, SHIFT, LAYER, false, 256, 4>, p.rows, threads(2), 0, 0, stream, p);
-  if (pieces <= 1024) return launch_dependent(block_norm_kernel<XT, YT, 8, 2, SHIFT, LAYER, false, 512, 2>, p.rows, threads(2), 0, 0, stream, p);
-  return launch_dependent(block_norm_kernel<XT, YT, 8, 4, SHIFT, LAYER, false, 512, 1>, p.rows, threads(4), 0, 0, stream, p);
+  if (pieces <= 32) return launch_dependent(block_norm_kernel<XT, YT, 8, 1, SHIFT, LAYER, true, false, 256, 5>, groups, 256, 0, 0, stream, p);
+  if (pieces <= 64) return launch_dependent(block_norm_kernel<XT, YT, 8, 2, SHIFT, LAYER, true, false, 256, 4>, groups, 256, 0, 0, stream, p);
+  const int nv = pieces <= 1024 ? 2 : 4;
+  const int smem = threads(nv) * nv * 8 * static_cast<int>(sizeof(XT) + sizeof(YT) * (SHIFT ? 6 : 1));
+  if (p.rows >= kRingRows && pieces >= kRingPieces && smem <= 110 * 1024) {
+    static std::atomic<int> known[3][17];
+    if (pieces <= 512) return launch_ring(block_norm_kernel<XT, YT, 8, 2, SHIFT, LAYER, false, true, 256, 4>, p, threads(2), smem, SHIFT, num_sms, known[0], stream);
+    if (pieces <= 1024) return launch_ring(block_norm_kernel<XT, YT, 8, 2, SHIFT, LAYER, false, true, 512, 2>, p, threads(2), smem, SHIFT, num_sms, known[1], stream);
+    return launch_ring(block_norm_kernel<XT, YT, 8, 4, SHIFT, LAYER, false, true, 512, 1>, p, threads(4), smem, SHIFT, num_sms, known[2], stream);
+  }
+  if (pieces <= 512) return launch_dependent(block_norm_kernel<XT, YT, 8, 2, SHIFT, LAYER, false, false, 256, 4>, p.rows, threads(2), 0, 0, stream, p);
+  if (pieces <= 1024) return launch_dependent(block_norm_kernel<XT, YT, 8, 2, SHIFT, LAYER, false, false, 512, 2>, p.rows, threads(2), 0, 0, stream, p);
+  return launch_dependent(block_norm_kernel<XT, YT, 8, 4, SHIFT, LAYER, false, false, 512, 1>, p.rows, threads(4), 0, 0, stream, p);
 }
 template <class XT, class YT, bool LAYER>
-int launch_layer(const NormParams& p, bool vec, bool shift, cudaStream_t stream) {
-  if (vec) return launch_pieces<XT, YT, false, LAYER>(p, stream);
-  if (shift && p.cols <= 16370) return launch_pieces<XT, YT, true, LAYER>(p, stream);
-  if (p.cols <= 1024) return launch_dependent(block_norm_kernel<XT, YT, 1, 4, false, LAYER, false, 256, 1>, p.rows, (p.cols + 127) / 128 * 32, 0, 0, stream, p);
-  return launch_dependent(block_norm_kernel<XT, YT, 1, 16, false, LAYER, false, 1024, 1>, p.rows, (p.cols + 511) / 512 * 32, 0, 0, stream, p);
+int launch_layer(const NormParams& p, bool vec, bool shift, int num_sms, cudaStream_t stream) {
+  if (vec) return launch_pieces<XT, YT, false, LAYER>(p, num_sms, stream);
+  if (shift && p.cols <= 16370) return launch_pieces<XT, YT, true, LAYER>(p, num_sms, stream);
+  if (p.cols <= 1024) return launch_dependent(block_norm_kernel<XT, YT, 1, 4, false, LAYER, false, false, 256, 1>, p.rows, (p.cols + 127) / 128 * 32, 0, 0, stream, p);
+  return launch_dependent(block_norm_kernel<XT, YT, 1, 16, false, LAYER, false, false, 1024, 1>, p.rows, (p.cols + 511) / 512 * 32, 0, 0, stream, p);
 }
 template <class XT, class YT>
-int launch_types(const NormParams& p, bool vec, bool shift, cudaStream_t stream) {
-  return p.layer ? launch_layer<XT, YT, true>(p, vec, shift, stream) : launch_layer<XT, YT, false>(p, vec, shift, stream);
+int launch_types(const NormParams& p, bool vec, bool shift, int num_sms, cudaStream_t stream) {
+  return p.layer ? launch_layer<XT, YT, true>(p, vec, shift, num_sms, stream) : launch_layer<XT, YT, false>(p, vec, shift, num_sms, stream);
 }
 
 }  // namespace
@@ -349,12 +463,12 @@ int launch_block_norm(const NormArgs& a, cudaStream_t stream) {
                      bases % 16 == 0 && ((reinterpret_cast<uintptr_t>(a.x) | reinterpret_cast<uintptr_t>(a.r)) % (a.x_type == 2 ? 32 : 16)) == 0 &&
                      (a.y_type != 2 || bases % 32 == 0) && (!gate_vec || reinterpret_cast<uintptr_t>(a.gate) % 16 == 0);
   if (a.x_type == 2) {
-    if (a.y_type == 2) return launch_types<float, float>(p, vec, shift, stream);
-    if (a.y_type == kBF16) return launch_types<float, __nv_bfloat16>(p, vec, shift, stream);
-    return launch_types<float, __half>(p, vec, shift, stream);
+    if (a.y_type == 2) return launch_types<float, float>(p, vec, shift, a.num_sms, stream);
+    if (a.y_type == kBF16) return launch_types<float, __nv_bfloat16>(p, vec, shift, a.num_sms, stream);
+    return launch_types<float, __half>(p, vec, shift, a.num_sms, stream);
   }
-  if (a.x_type == kBF16) return launch_types<__nv_bfloat16, __nv_bfloat16>(p, vec, shift, stream);
-  return launch_types<__half, __half>(p, vec, shift, stream);
+  if (a.x_type == kBF16) return launch_types<__nv_bfloat16, __nv_bfloat16>(p, vec, shift, a.num_sms, stream);
+  return launch_types<__half, __half>(p, vec, shift, a.num_sms, stream);
 }
 
 }  // namespace sfb200

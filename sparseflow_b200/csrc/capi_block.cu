@@ -107,13 +107,15 @@ int sfb200_block_norm(const void* x, int64_t ld_x, const void* y, int64_t ld_y, 
                       const void* post_bias, const void* gate, int64_t ld_gate, int gate_rows, int gate_cols, void* r, int64_t ld_r, void* h,
                       int64_t ld_h, int rows, int cols, int x_type, int y_type, float scale, float eps, float post_eps, int layer, void* stream) {
   int err = kOk;
-  if (!device_state(&err)) return err;
+  DeviceState* s = device_state(&err);
+  if (!s) return err;
   NormArgs a{};
   a.x = x; a.y = y; a.weight = weight; a.bias = bias; a.post_weight = post_weight; a.post_bias = post_bias; a.gate = gate;
   a.r = r; a.h = h;
   a.ld_x = ld_x; a.ld_y = ld_y; a.ld_r = ld_r; a.ld_h = ld_h; a.ld_gate = ld_gate;
   a.rows = rows; a.cols = cols; a.gate_rows = gate_rows; a.gate_cols = gate_cols;
   a.x_type = x_type; a.y_type = y_type;
+  a.num_sms = s->num_sms;
   a.scale = scale; a.eps = eps; a.post_eps = post_eps; a.layer = layer;
   return launch_block_norm(a, static_cast<cudaStream_t>(stream));
 }

@@ -196,6 +196,7 @@ struct NormArgs {
   int x_type, y_type;      // 0 f16, 1 bf16, 2 f32: x and r; everything else.  Equal, or x_type 2
   float scale, eps, post_eps;
   int layer;               // 0 rms, 1 layer norm
+  int num_sms;
 };
 constexpr int kNormMaxCols = 16384;
 int launch_block_norm(const NormArgs& a, cudaStream_t stream);

@@ -50,6 +50,21 @@ def test_gates_and_rows(rows, gates, H, post):
     _run(x, y, weight=None, post_weight=pw, post_bias=pw)      # no second norm
 
 
+@pytest.mark.parametrize("H", [2056, 2057, 4096, 4099, 8192, 8185, 12345, 16368, 16370])
+@pytest.mark.parametrize("kind,dt,stream", [("rms", "bf16", "f32"), ("layer", "f16", "f16"), ("rms", "f32", "f32")])
+def test_more_rows_than_blocks(H, kind, dt, stream):
+    """Blocks that stay and fetch their next row while they reduce one; the last row ends inside a piece."""
+    g = gen(H)
+    t, n = DT[dt], 1503
+    x, y = randn(g, n, H, dtype=DT[stream]), randn(g, n, H, dtype=t)
+    v = [randn(g, H, dtype=t) for _ in range(4)]
+    _run(x, y, kind, weight=v[0], bias=v[1], post_weight=v[2], post_bias=v[3], gate=v[1])
+    _run(x, y, kind, weight=v[0], gate=randn(g, 3, H, dtype=t))
+    _run(x, y, kind, post_weight=v[2])
+    _run(x, y, kind)
+    _run(x, None, kind, weight=v[0])
+
+
 @pytest.mark.parametrize("H,pitch,at", [(64, 80, 0), (64, 80, 3), (1001, 1009, 0), (1001, 1001, 0), (1000, 1003, 1), (4097, 4105, 0)])
 def test_strides(H, pitch, at):
     g = gen(H + pitch)
