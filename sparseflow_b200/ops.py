@@ -310,26 +310,29 @@ def _on_device_of(x: torch.Tensor, t: Optional[torch.Tensor], name: str) -> None
         raise ValueError(f"{name} must be a CUDA tensor on {x.device}, got {t.device}")
 
 
-def _rows2d(t: torch.Tensor, name: str) -> torch.Tensor:
-    """2-D with unit inner stride; rows may be strided (a view that is not so is copied)."""
+def _rows2d(t: torch.Tensor, name: str) -> tuple:
+    """(t, row pitch in elements): 2-D with unit inner stride, rows may be strided (a view that is not so is copied)."""
     if t.dim() != 2:
         raise ValueError(f"{name} must be 2D, got {t.dim()}D")
-    if (t.stride(1) != 1 and t.shape[1] > 1) or (t.shape[0] > 1 and t.stride(0) < t.shape[1]):
-        return t.contiguous()
-    return t
+    if not t.is_contiguous() and ((t.stride(1) != 1 and t.shape[1] > 1) or (t.shape[0] > 1 and t.stride(0) < t.shape[1])):
+        t = t.contiguous()
+    return t, _pitch(t)
 
 
-def _rows16(t: torch.Tensor, name: str) -> torch.Tensor:
+def _rows16(t: torch.Tensor, name: str) -> tuple:
     """``_rows2d`` with what 16-byte accesses need: row pitch a multiple of 8 elements, 16-byte aligned base."""
-    t = _rows2d(t, name)
-    if t.data_ptr() % 16 or (t.shape[0] > 1 and t.stride(0) % 8):
+    t, pitch = _rows2d(t, name)
+    if t.data_ptr() % 16 or pitch % 8:
         t = t.clone(memory_format=torch.contiguous_format)
-    return t
+        pitch = _pitch(t)
+    return t, pitch
 
 
 def _pitch(t: torch.Tensor) -> int:
     """Row pitch in elements (of one row: its length, whatever its stride says)."""
-    return t.stride(0) if t.shape[0] > 1 else max(t.shape[1], 1)
+    if t.is_contiguous():
+        return t.size(1)
+    return t.stride(0) if t.size(0) > 1 else t.size(1)
 
 
 def _check_out(out: torch.Tensor, like: torch.Tensor, shape: tuple, dtype: torch.dtype) -> None:
@@ -406,20 +409,19 @@ def moe_route(logits: torch.Tensor, top_k: int, renormalize: bool = True) -> Rou
     dt = _DT3.get(logits.dtype)
     if dt is None:
         raise ValueError(f"logits must be float16, bfloat16 or float32, got {logits.dtype}")
-    logits = _rows2d(logits, "logits")
+    logits, ld = _rows2d(logits, "logits")
     n, E = logits.shape
     if not 1 <= E <= 1024:
         raise ValueError(f"experts must be 1 .. 1024, got {E}")
     if not 1 <= top_k <= min(32, E):
         raise ValueError(f"top_k must be 1 .. {min(32, E)}, got {top_k}")
     L = _lib.lib()
-    weights = logits.new_empty((n, top_k), dtype=torch.float32)
-    chosen = logits.new_empty((n, top_k), dtype=torch.int32)
-    slots = logits.new_empty((n, top_k), dtype=torch.int32)
-    rows = logits.new_empty(n * top_k, dtype=torch.int32)
+    # one allocation for the four results of n * top_k words: an allocation costs as much host time as the kernel takes
+    weights, chosen, slots, rows = logits.new_empty((4, n, top_k), dtype=torch.int32).unbind(0)
+    weights, rows = weights.view(torch.float32), rows.view(-1)
     offsets = logits.new_empty(E + 1, dtype=torch.int32)
     work = logits.new_empty(L.sfb200_group_workspace_bytes(E), dtype=torch.uint8) if n > 32 else None
-    rc = L.sfb200_moe_route(logits.data_ptr(), _pitch(logits), n, E, top_k, dt, 1 if renormalize else 0, weights.data_ptr(), chosen.data_ptr(),
+    rc = L.sfb200_moe_route(logits.data_ptr(), ld, n, E, top_k, dt, 1 if renormalize else 0, weights.data_ptr(), chosen.data_ptr(),
                             offsets.data_ptr(), rows.data_ptr(), slots.data_ptr(), _ptr(work), _stream_of(logits.get_device()))
     if rc:
         _lib.check("sfb200_moe_route", rc)
@@ -519,7 +521,7 @@ def _grouped_args(x: torch.Tensor, cw: CompressedExperts, groups: RowGroups, gat
             raise ValueError(f"grouping is of {total // groups.per_row} rows, x has {x.shape[0]}")
     elif x.shape[0] != total:
         raise ValueError(f"grouping has {total} places, x has {x.shape[0]} rows (gather=True reads x through the grouping)")
-    return _rows16(x, "x"), total
+    return *_rows16(x, "x"), total
 
 
 def _grouped_scratch(x: torch.Tensor, total: int, cw: CompressedExperts) -> Optional[torch.Tensor]:
@@ -534,7 +536,7 @@ def grouped_sparse_gemm(x: torch.Tensor, cw: CompressedExperts, groups: RowGroup
 
     ``x`` holds a row per place in the order of ``groups``; with ``gather`` a row per token, read through ``groups.rows``.  Rows of the
     result behind the last group are left as they were (in a fresh result: undefined).  ``out`` shares no memory with ``x``."""
-    x, total = _grouped_args(x, cw, groups, gather)
+    x, ldx, total = _grouped_args(x, cw, groups, gather)
     if act not in ACT:
         raise ValueError(f"unknown activation {act!r}")
     if cw.gate_up:
@@ -548,7 +550,7 @@ def grouped_sparse_gemm(x: torch.Tensor, cw: CompressedExperts, groups: RowGroup
     if total == 0:
         return out
     scratch = _grouped_scratch(x, total, cw) if gather else None
-    rc = _lib.lib().sfb200_grouped_sparse_gemm(x.data_ptr(), _pitch(x), x.shape[0], groups.rows.data_ptr() if gather else None, _ptr(scratch),
+    rc = _lib.lib().sfb200_grouped_sparse_gemm(x.data_ptr(), ldx, x.shape[0], groups.rows.data_ptr() if gather else None, _ptr(scratch),
                                                cw.values.data_ptr(), cw.meta.data_ptr(), out.data_ptr(), _pitch(out), total, cw.experts, cw.rows,
                                                cw.K, _dt(x), _ptr(bias), ACT[act], groups.offsets.data_ptr(), _stream_of(x.get_device()))
     if rc:
@@ -562,7 +564,7 @@ def grouped_sparse_gemm_swiglu(x: torch.Tensor, cw_gu: CompressedExperts, groups
                                out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """h[place] = silu(x . Wg_e^T + gate_bias[e]) * (x . Wu_e^T + up_bias[e]) from the fused gate|up weights; ``x``, ``gather`` and
     the rows behind the last group as in ``grouped_sparse_gemm``."""
-    x, total = _grouped_args(x, cw_gu, groups, gather)
+    x, ldx, total = _grouped_args(x, cw_gu, groups, gather)
     if not cw_gu.gate_up:
         raise ValueError("weights were not built with compress_gate_up_experts")
     I = cw_gu.rows // 2
@@ -576,7 +578,7 @@ def grouped_sparse_gemm_swiglu(x: torch.Tensor, cw_gu: CompressedExperts, groups
     if total == 0:
         return out
     scratch = _grouped_scratch(x, total, cw_gu) if gather else None
-    rc = _lib.lib().sfb200_grouped_sparse_gemm_swiglu(x.data_ptr(), _pitch(x), x.shape[0], groups.rows.data_ptr() if gather else None,
+    rc = _lib.lib().sfb200_grouped_sparse_gemm_swiglu(x.data_ptr(), ldx, x.shape[0], groups.rows.data_ptr() if gather else None,
                                                       _ptr(scratch), cw_gu.values.data_ptr(), cw_gu.meta.data_ptr(), out.data_ptr(), _pitch(out),
                                                       total, cw_gu.experts, I, cw_gu.K, _dt(x), _ptr(gate_bias), _ptr(up_bias),
                                                       groups.offsets.data_ptr(), _stream_of(x.get_device()))
@@ -591,32 +593,35 @@ def moe_combine(y: torch.Tensor, slots: torch.Tensor, weights: torch.Tensor, res
     """out[t] = residual[t] + sum_j weights[t, j] * y[slots[t, j]], in 32 bits, rounded once; a slot of -1 adds nothing.
     ``out`` may be ``residual``."""
     dt = _dt(y)
-    y = _rows2d(y, "y")
-    if slots.dim() != 2 or slots.shape != weights.shape or slots.dtype != torch.int32 or weights.dtype != torch.float32 or not slots.shape[1]:
+    y, ld_y = _rows2d(y, "y")
+    if slots.dim() != 2 or slots.shape != weights.shape or slots.dtype != torch.int32 or weights.dtype != torch.float32:
         raise ValueError("slots must be [tokens, top_k] int32 and weights the same shape in float32")
-    _on_device_of(y, slots, "slots")
-    _on_device_of(y, weights, "weights")
+    dev = y.get_device()
+    if slots.get_device() != dev or weights.get_device() != dev:
+        _on_device_of(y, slots, "slots")
+        _on_device_of(y, weights, "weights")
     n, k = slots.shape
-    H = y.shape[1]
-    if not H:
-        raise ValueError("y has no columns")
+    rows, H = y.shape
+    if not H or not k:
+        raise ValueError(f"nothing to add up: y is {tuple(y.shape)}, slots {tuple(slots.shape)}")
     ld_res = 0
     if residual is not None:
         _on_device_of(y, residual, "residual")
         if tuple(residual.shape) != (n, H) or residual.dtype != y.dtype:
             raise ValueError(f"residual must be [{n}, {H}] {y.dtype}")
-        residual = _rows2d(residual, "residual")
-        ld_res = _pitch(residual)
-    slots, weights = slots.contiguous(), weights.contiguous()
+        residual, ld_res = _rows2d(residual, "residual")
+    if not (slots.is_contiguous() and weights.is_contiguous()):
+        slots, weights = slots.contiguous(), weights.contiguous()
     if out is None:
-        out = y.new_empty((n, H))
+        out, ld_out = y.new_empty((n, H)), H
     else:
         _check_out(out, y, (n, H), y.dtype)
         _check_apart(out, y, "y")
         if residual is not None:
             _check_apart(out, residual, "residual", same=True)
-    rc = _lib.lib().sfb200_moe_combine(y.data_ptr(), _pitch(y), y.shape[0], slots.data_ptr(), weights.data_ptr(), _ptr(residual), ld_res,
-                                       out.data_ptr(), _pitch(out), n, k, H, dt, _stream_of(y.get_device()))
+        ld_out = _pitch(out)
+    rc = _lib.lib().sfb200_moe_combine(y.data_ptr(), ld_y, rows, slots.data_ptr(), weights.data_ptr(), _ptr(residual), ld_res, out.data_ptr(), ld_out,
+                                       n, k, H, dt, _stream_of(dev))
     if rc:
         _lib.check("sfb200_moe_combine", rc)
     return out
@@ -640,7 +645,7 @@ def block_norm(x: torch.Tensor, y: Optional[torch.Tensor] = None, *, weight: Opt
     xt = _DT3.get(x.dtype)
     if xt is None:
         raise ValueError(f"x must be float16, bfloat16 or float32, got {x.dtype}")
-    x = _rows2d(x, "x")
+    x, ld_x = _rows2d(x, "x")
     n, H = x.shape
     if not 1 <= H <= 16384:
         raise ValueError(f"cols must be 1 .. 16384, got {H}")
@@ -656,11 +661,13 @@ def block_norm(x: torch.Tensor, y: Optional[torch.Tensor] = None, *, weight: Opt
     if (bias is not None and weight is None) or (post_bias is not None and post_weight is None):
         raise ValueError("a bias needs its weight")
 
+    dev = x.get_device()
+
     def vector(v, name):
         if v is None:
             return None
-        _on_device_of(x, v, name)
-        if v.dtype != dtype or tuple(v.shape) != (H,):
+        if v.dtype is not dtype or v.dim() != 1 or v.size(0) != H or v.get_device() != dev:
+            _on_device_of(x, v, name)
             raise ValueError(f"{name} must be [{H}] {dtype}, got {tuple(v.shape)} {v.dtype}")
         return v if v.is_contiguous() else v.contiguous()
 
@@ -674,8 +681,7 @@ def block_norm(x: torch.Tensor, y: Optional[torch.Tensor] = None, *, weight: Opt
         _on_device_of(x, y, "y")
         if y.shape != x.shape:
             raise ValueError(f"y must be {tuple(x.shape)}, got {tuple(y.shape)}")
-        y = _rows2d(y, "y")
-        ld_y = _pitch(y)
+        y, ld_y = _rows2d(y, "y")
     if gate is not None:
         _on_device_of(x, gate, "gate")
         if gate.dtype != dtype:
@@ -684,13 +690,13 @@ def block_norm(x: torch.Tensor, y: Optional[torch.Tensor] = None, *, weight: Opt
             gate = gate.unsqueeze(0)
         if gate.dim() != 2 or gate.shape[1] not in (1, H) or not gate.shape[0] or n % gate.shape[0]:
             raise ValueError(f"gate must be [{H}], or [g, {H}] or [g, 1] with g dividing {n} rows, got {tuple(gate.shape)}")
-        gate = _rows2d(gate, "gate")
-        ld_gate, (gate_rows, gate_cols) = _pitch(gate), gate.shape
+        gate, ld_gate = _rows2d(gate, "gate")
+        gate_rows, gate_cols = gate.shape
     r = x.new_empty((n, H)) if y is not None else None
     h = (x if y is None else y).new_empty((n, H), dtype=dtype) if weight is not None else None
-    rc = _lib.lib().sfb200_block_norm(x.data_ptr(), _pitch(x), _ptr(y), ld_y, _ptr(weight), _ptr(bias), _ptr(post_weight), _ptr(post_bias), _ptr(gate),
+    rc = _lib.lib().sfb200_block_norm(x.data_ptr(), ld_x, _ptr(y), ld_y, _ptr(weight), _ptr(bias), _ptr(post_weight), _ptr(post_bias), _ptr(gate),
                                       ld_gate, gate_rows, gate_cols, _ptr(r), H, _ptr(h), H, n, H, xt, yt, scale, eps,
-                                      eps if post_eps is None else post_eps, 1 if kind == "layer" else 0, _stream_of(x.get_device()))
+                                      eps if post_eps is None else post_eps, 1 if kind == "layer" else 0, _stream_of(dev))
     if rc:
         _lib.check("sfb200_block_norm", rc)
     return (x if r is None else r), h
@@ -755,7 +761,7 @@ def lora_add(y: torch.Tensor, x: torch.Tensor, bank: LoraBank, groups: RowGroups
     _on_device_of(y, x, "x")
     _on_device_of(y, bank.a, "adapters")
     _on_device_of(y, groups.offsets, "groups")
-    x = _rows16(x, "x")
+    x, ld_x = _rows16(x, "x")
     if out is None:
         out = y.new_empty((n, bank.N))
     else:
@@ -766,15 +772,17 @@ def lora_add(y: torch.Tensor, x: torch.Tensor, bank: LoraBank, groups: RowGroups
         return out
     into = out
     if out is y:
-        y = out = _rows16(y, "y")
+        y, ld_y = _rows16(y, "y")
+        out, ld_out = y, ld_y
     else:
-        y = _rows16(y, "y")
-        if out.data_ptr() % 16 or _pitch(out) % 8:
-            out = y.new_empty((n, bank.N))
+        y, ld_y = _rows16(y, "y")
+        ld_out = _pitch(out)
+        if out.data_ptr() % 16 or ld_out % 8:
+            out, ld_out = y.new_empty((n, bank.N)), bank.N
     L = _lib.lib()
     work = y.new_empty(L.sfb200_lora_workspace_bytes(n, bank.rank), dtype=torch.uint8)
-    rc = L.sfb200_lora_add(y.data_ptr(), _pitch(y), x.data_ptr(), _pitch(x), bank.a.data_ptr(), bank.b.data_ptr(), bank.scales.data_ptr(),
-                           out.data_ptr(), _pitch(out), n, bank.adapters, bank.rank, bank.K, bank.N, _dt(y), groups.offsets.data_ptr(),
+    rc = L.sfb200_lora_add(y.data_ptr(), ld_y, x.data_ptr(), ld_x, bank.a.data_ptr(), bank.b.data_ptr(), bank.scales.data_ptr(),
+                           out.data_ptr(), ld_out, n, bank.adapters, bank.rank, bank.K, bank.N, _dt(y), groups.offsets.data_ptr(),
                            groups.rows.data_ptr(), groups.slots.data_ptr(), work.data_ptr(), _stream_of(y.get_device()))
     if rc:
         _lib.check("sfb200_lora_add", rc)
