@@ -22,6 +22,7 @@
 
 #include <atomic>
 
+#include "device_state.h"
 #include "kernels.h"
 #include "launch.h"
 #include "sm100_ptx.cuh"
@@ -380,12 +381,14 @@ __global__ void __launch_bounds__(MAXT, MINB) block_norm_kernel(const NormParams
 
 // Rows and pieces of a row from which blocks stay: with a row or two each there is nothing to fetch ahead, and eight or more short rows per SM cover each
 // other (16384 x 1024 f32 38 us, with the ring 44; 3000 x 1001 8.6 and 10.6; 4096 x 8192 f32 83 and 78, 8192 x 4097 layer norms 160 and 122).
-constexpr int kRingRows = 4 * 148, kRingPieces = 257;
+constexpr int kRingRows = 4 * 148, kRingPieces = 257, kRingSizes = 17;
 
 template <class Kernel>
 int launch_ring(Kernel kernel, const NormParams& p, int threads, int smem, bool shift, int num_sms, std::atomic<int>* known, cudaStream_t stream) {
-  // blocks per SM, asked for once per block size and shared-memory size (both change rarely)
-  std::atomic<int>& slot = known[threads / 32];
+  // blocks per SM, asked for once per device, block size and shared-memory size (they change rarely)
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= kMaxDevices) return kErrCuda;
+  std::atomic<int>& slot = known[dev * kRingSizes + threads / 32];
   int per_sm = slot.load(std::memory_order_relaxed);
   if (per_sm / 16 != smem / 16) {
     int n = 0;
@@ -410,7 +413,7 @@ int launch_pieces(const NormParams& p, int num_sms, cudaStream_t stream) {
   const int nv = pieces <= 1024 ? 2 : 4;
   const int smem = threads(nv) * nv * 8 * static_cast<int>(sizeof(XT) + sizeof(YT) * (SHIFT ? 6 : 1));
   if (p.rows >= kRingRows && pieces >= kRingPieces && smem <= 110 * 1024) {
-    static std::atomic<int> known[3][17];
+    static std::atomic<int> known[3][kMaxDevices * kRingSizes];
     if (pieces <= 512) return launch_ring(block_norm_kernel<XT, YT, 8, 2, SHIFT, LAYER, false, true, 256, 4>, p, threads(2), smem, SHIFT, num_sms, known[0], stream);
     if (pieces <= 1024) return launch_ring(block_norm_kernel<XT, YT, 8, 2, SHIFT, LAYER, false, true, 512, 2>, p, threads(2), smem, SHIFT, num_sms, known[1], stream);
     return launch_ring(block_norm_kernel<XT, YT, 8, 4, SHIFT, LAYER, false, true, 512, 1>, p, threads(4), smem, SHIFT, num_sms, known[2], stream);
