@@ -39,6 +39,7 @@ struct LoraParams {
   int64_t ld_y, ld_x, ld_out;
   int n, groups, K, N, tile, tiles, copy_blocks;      // n: rows; tile: rows per tile; tiles: upper bound of their number
   int splits, slice;                                  // slices of K (blocks of a cluster), of `slice` values
+  int tiles_first;                                    // lora_up's grid: tiles along x, columns along y (more tiles than y takes)
 };
 
 // Tile number -> its group and rows [first, first + count); false: no such tile (and first = number of tiles).  Executed by whole warps.
@@ -389,15 +390,16 @@ template <bool BF16, int NF>
 __global__ void __launch_bounds__(kUpWarps * 32) lora_up_kernel(const LoraParams p, int cols_per_block) {
   constexpr int R = 8 * NF;
   using S = RankStep<R>;
-  const int c_begin = blockIdx.x * cols_per_block, c_end = min(p.N, c_begin + cols_per_block);
-  if (static_cast<int>(blockIdx.y) >= p.tiles) {
+  const int tile = p.tiles_first ? blockIdx.x : blockIdx.y;
+  const int c_begin = (p.tiles_first ? blockIdx.y : blockIdx.x) * cols_per_block, c_end = min(p.N, c_begin + cols_per_block);
+  if (tile >= p.tiles) {
     dependency_wait();
     dependency_trigger();
-    copy_rows(p, blockIdx.y - p.tiles, c_begin, c_end);
+    copy_rows(p, tile - p.tiles, c_begin, c_end);
     return;
   }
   int group = 0, first = 0, count = 0;
-  if (!find_tile(p, blockIdx.y, group, first, count)) {
+  if (!find_tile(p, tile, group, first, count)) {
     dependency_wait();
     dependency_trigger();
     return;
@@ -459,15 +461,16 @@ __global__ void __launch_bounds__(kUpWarps * 32) lora_up_tile_kernel(const LoraP
   extern __shared__ __align__(128) uint8_t smem[];
   constexpr int R = 8 * NF, B_BYTES = kUpCols * R * 2, Y_BYTES = kUpWarps * 32 * MF * 2 * 16, STAGE = B_BYTES + Y_BYTES;
   using S = RankStep<R>;
-  const int c_begin = blockIdx.x * cols, c_end = min(p.N, c_begin + cols);
-  if (static_cast<int>(blockIdx.y) >= p.tiles) {
+  const int tile = p.tiles_first ? blockIdx.x : blockIdx.y;
+  const int c_begin = (p.tiles_first ? blockIdx.y : blockIdx.x) * cols, c_end = min(p.N, c_begin + cols);
+  if (tile >= p.tiles) {
     dependency_wait();
     dependency_trigger();
-    copy_rows(p, blockIdx.y - p.tiles, c_begin, c_end);
+    copy_rows(p, tile - p.tiles, c_begin, c_end);
     return;
   }
   int group = 0, first = 0, count = 0;
-  if (!find_tile(p, blockIdx.y, group, first, count)) {
+  if (!find_tile(p, tile, group, first, count)) {
     dependency_wait();
     dependency_trigger();
     return;
@@ -626,7 +629,6 @@ int launch_rank(LoraParams p, int num_sms, cudaStream_t stream) {
     p.tiles = (p.n + p.tile - 1) / p.tile + (p.groups < p.n ? p.groups : p.n);
   }
   p.copy_blocks = p.out == p.y ? 0 : (p.n + 31) / 32;
-  if (p.tiles + p.copy_blocks > 65535) return kErrInvalid;      // rows: above two million
   int cols = 128;
   if (l.tiled) {
     // about six blocks of work per SM: a block begins with a chain of loads (its tile, its rows, their u) of about 2 us
@@ -634,7 +636,10 @@ int launch_rank(LoraParams p, int num_sms, cudaStream_t stream) {
     cols = static_cast<int>(tiles * p.N / (6 * num_sms));
     cols = cols < 128 ? 128 : (cols + 63) / 64 * 64;
   }
-  const dim3 grid((p.N + cols - 1) / cols, p.tiles + p.copy_blocks, 1);
+  const int across = (p.N + cols - 1) / cols, along = p.tiles + p.copy_blocks;
+  p.tiles_first = along > 65535;
+  if (p.tiles_first && across > 65535) return kErrInvalid;
+  const dim3 grid(p.tiles_first ? along : across, p.tiles_first ? across : along, 1);
   if (!l.tiled) return launch_dependent(lora_up_kernel<BF16, NF>, grid, kUpWarps * 32, 0, 0, stream, p, cols);
   constexpr int smem = kUpStages * (kUpCols * R * 2 + kUpWarps * 32 * MF * 2 * 16);
   static bool set[16] = {};

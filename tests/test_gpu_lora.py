@@ -69,6 +69,18 @@ def test_strides(n, A):
     assert torch.equal(ops.lora_add(y, x, bank, groups, out=out), ref) and (wide[:, :8] == 0).all()
 
 
+def test_more_rows_than_a_grid_dimension():
+    """2.2 million rows (tiles and copies above 65535), in place and not; compared with the same rows in two calls."""
+    n, g = 2_200_000, gen(12)
+    x, y, a, b, s, ids = _case(g, n, 2, 8, 8, 8, torch.bfloat16)
+    bank = ops.LoraBank(a, b, s)
+    out = ops.lora_add(y, x, bank, ops.group_rows(ids, 2))
+    for part in (slice(0, 3000), slice(n - 3000, n)):
+        close(out[part], *_reference(x[part], y[part], a, b, s, ids[part]))
+    assert torch.equal(out[ids < 0], y[ids < 0])
+    assert torch.equal(ops.lora_add(y, x, bank, ops.group_rows(ids, 2), out=y), out)
+
+
 def test_large_and_small_products_of_f16():
     """u beyond the range of f16 and far below it: the row is scaled by a power of two."""
     g = gen(2)
