@@ -308,13 +308,17 @@ int plan_grouped(int total, int experts, int n_out, int K, bool gather, int num_
   static const int variants[] = {32, 64, 1128, 1240, 2128, 2240};
   int best = 0;
   double cost = 1e300;
+  // the tables of tiles, 8 bytes per expert, stand beside the ring in shared memory: 2128 leaves 1.8 KB for them, the other forms hold kMaxExperts
+  auto fits = [&](int v) { return v != 2128 || experts <= 220; };
   for (int v : variants) {
+    if (!fits(v)) continue;
     const double c = grouped_cost(v, gather, total, experts, n_out, K, num_sms);
     if (c < cost) { cost = c; best = v; }
   }
   if (!gather) return best;
   const double copy = 3.0 + static_cast<double>(total) * K * 4.0 / 7.4e6;
   for (int v : variants) {
+    if (!fits(v)) continue;
     const double c = copy + grouped_cost(v, false, total, experts, n_out, K, num_sms);
     if (c < cost) { cost = c; best = 10000 + v; }
   }

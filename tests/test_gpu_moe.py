@@ -131,6 +131,22 @@ def test_grouped_swiglu(form, variant, sizes, dt, I, K, biased):
     close(out, silu * up, 1.1 * gs * up.abs() + silu.abs() * us + gs * us + 2.0 ** -18 * (silu * up).abs())
 
 
+@pytest.mark.parametrize("per_expert", [0.2, 3, 60, 130])
+@pytest.mark.parametrize("gather", [False, True])
+def test_many_experts(per_expert, gather):
+    """1024 experts: whatever form the plan names, its tables fit."""
+    E, N, K = 1024, 72, 64
+    g = gen(int(per_expert * 10))
+    w = _weights(g, E, N, K, torch.bfloat16)
+    ids = torch.randint(0, E, (int(E * per_expert),), generator=g, device="cuda")
+    groups = ops.group_rows(ids, E)
+    x = randn(g, ids.numel(), K, dtype=torch.bfloat16)
+    y = ops.grouped_sparse_gemm(x, ops.compress_experts(w), groups, gather=gather)
+    assert ops.device_status() == 0
+    rows, sizes = groups.rows.long(), groups.offsets.diff().tolist()
+    close(y, *_reference(x[rows] if gather else x, w, sizes, None))
+
+
 @pytest.mark.parametrize("act", ["none", "relu", "silu", "gelu"])
 def test_grouped_activations(act):
     g = gen(5)
