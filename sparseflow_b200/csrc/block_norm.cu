@@ -13,7 +13,7 @@
 // pieces at the ends of a row are stored value by value, and weights, which begin at column 0, are shifted by m from two pieces.
 // Value by value throughout where the tensors' rows do not lie alike in their pieces.
 // Measured: 4096 x 8192 (f32 stream, bf16, norm on both sides) 78 us (5.2 TB/s), 16384 x 2048 bf16 58 us (4.6 TB/s; issue-bound: 50 instructions
-// a piece), 8192 x 4097 layer norms 122 us, 24 x 4096 2.8 us (latency).
+// a piece), 8192 x 4097 layer norms 122 us, 24 x 4096 2.7 us (latency).
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -410,6 +410,10 @@ int launch_pieces(const NormParams& p, int num_sms, cudaStream_t stream) {
   const int groups = (p.rows + 7) / 8;
   if (pieces <= 32) return launch_dependent(block_norm_kernel<XT, YT, 8, 1, SHIFT, LAYER, true, false, 256, 5>, groups, 256, 0, 0, stream, p);
   if (pieces <= 64) return launch_dependent(block_norm_kernel<XT, YT, 8, 2, SHIFT, LAYER, true, false, 256, 4>, groups, 256, 0, 0, stream, p);
+  // a row or less per SM is latency: a piece per thread (24 rows of 1024 1.74 us, with two 2.36; of 4096 2.26 and 2.66; of 8192, where the sums of
+  // 32 warps are added, 4.2 and 3.7)
+  if (p.rows <= num_sms && pieces <= 640)
+    return launch_dependent(block_norm_kernel<XT, YT, 8, 1, SHIFT, LAYER, false, false, 640, 1>, p.rows, threads(1), 0, 0, stream, p);
   const int nv = pieces <= 1024 ? 2 : 4;
   const int smem = threads(nv) * nv * 8 * static_cast<int>(sizeof(XT) + sizeof(YT) * (SHIFT ? 6 : 1));
   if (p.rows >= kRingRows && pieces >= kRingPieces && smem <= 110 * 1024) {
@@ -437,7 +441,7 @@ int launch_types(const NormParams& p, bool vec, bool shift, int num_sms, cudaStr
 }  // namespace
 
 int launch_block_norm(const NormArgs& a, cudaStream_t stream) {
-  if (a.rows < 0 || a.cols < 1 || a.cols > kNormMaxCols) return kErrInvalid;
+  if (a.rows < 0 || a.rows > 0x7fffffff - 4096 || a.cols < 1 || a.cols > kNormMaxCols) return kErrInvalid;
   if (a.rows == 0) return kOk;
   if (!a.x || (!a.r && !a.h) || (a.h && !a.weight) || (a.y && !a.r) || (!a.y && (a.r || a.gate || a.post_weight))) return kErrInvalid;
   if (a.ld_x < a.cols || (a.y && a.ld_y < a.cols) || (a.r && a.ld_r < a.cols) || (a.h && a.ld_h < a.cols)) return kErrInvalid;
