@@ -5,6 +5,7 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include "device_state.h"
 #include "kernels.h"
 #include "sm100_pair.cuh"
 #include "sm100_ptx.cuh"
@@ -12,7 +13,6 @@
 namespace sfb200 {
 
 constexpr int kMaxExperts = 1024;
-constexpr int kMaxDevicesGrouped = 16;
 
 struct GroupedParams {
   const uint32_t* meta;   // [experts][row_tiles][k_tiles][128][4]

@@ -5,7 +5,8 @@
 // (dependency_wait), which returns when the kernel before it has completed and its writes are visible.  Rules for the
 // kernels launched this way:
 //   * before dependency_wait nothing is read or written but launch parameters; the weights are only PREFETCHED into L2,
-//     which is right whoever wrote them last;
+//     which is right whoever wrote them last.  (The second kernel of a pair that one call launches may read there what the first does not write: by the
+//     rule on dependency_trigger below, all from before the first is complete when the second begins.  lora.cu does so.)
 //   * what a predecessor may have written is read with ordinary loads (or TMA / cp.async) after dependency_wait, never through
 //     the read-only path (__ldg, ld.global.nc, const __restrict__): that is for data nobody writes while the kernel runs, and
 //     this kernel is running while its predecessor writes;

@@ -21,6 +21,7 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include "device_state.h"
 #include "kernels.h"
 #include "launch.h"
 #include "sm100_ptx.cuh"
@@ -573,13 +574,13 @@ __global__ void __launch_bounds__(kUpWarps * 32) lora_up_tile_kernel(const LoraP
 }
 
 template <class Kernel>
-int allow_smem(Kernel kernel, int bytes, bool (&set)[16]) {
+int allow_smem(Kernel kernel, int bytes, bool (&set)[kMaxDevices]) {
   if (bytes <= 48 * 1024) return kOk;
   int dev = 0;
-  cudaGetDevice(&dev);
-  if (dev < 16 && set[dev]) return kOk;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= kMaxDevices) return kErrCuda;
+  if (set[dev]) return kOk;
   if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess) return kErrCuda;
-  if (dev < 16) set[dev] = true;
+  set[dev] = true;
   return kOk;
 }
 
@@ -613,12 +614,12 @@ int launch_rank(LoraParams p, int num_sms, cudaStream_t stream) {
   if (l.tiled) {
     constexpr int smem = kStages * (kTileRows + (R < 16 ? 16 : R)) * 128;
     static_assert(smem >= kTileRows * R * 4, "the partial sums fit the ring");
-    static bool set[16] = {};
+    static bool set[kMaxDevices] = {};
     if ((rc = allow_smem(lora_down_tile_kernel<BF16, NF>, smem, set)) != kOk) return rc;
     rc = launch_dependent(lora_down_tile_kernel<BF16, NF>, p.tiles * p.splits, 256, smem, p.splits, stream, p);
   } else {
     constexpr int smem = kDownWarps * 16 * R * 4;
-    static bool set[16] = {};
+    static bool set[kMaxDevices] = {};
     if ((rc = allow_smem(lora_down_kernel<BF16, 1, NF>, smem, set)) != kOk) return rc;
     rc = launch_dependent(lora_down_kernel<BF16, 1, NF>, p.tiles * p.splits, kDownWarps * 32, smem, p.splits, stream, p);
   }
@@ -642,7 +643,7 @@ int launch_rank(LoraParams p, int num_sms, cudaStream_t stream) {
   const dim3 grid(p.tiles_first ? along : across, p.tiles_first ? across : along, 1);
   if (!l.tiled) return launch_dependent(lora_up_kernel<BF16, NF>, grid, kUpWarps * 32, 0, 0, stream, p, cols);
   constexpr int smem = kUpStages * (kUpCols * R * 2 + kUpWarps * 32 * MF * 2 * 16);
-  static bool set[16] = {};
+  static bool set[kMaxDevices] = {};
   if ((rc = allow_smem(lora_up_tile_kernel<BF16, NF, MF>, smem, set)) != kOk) return rc;
   return launch_dependent(lora_up_tile_kernel<BF16, NF, MF>, grid, kUpWarps * 32, smem, 0, stream, p, cols);
 }
@@ -664,7 +665,7 @@ int launch_type(const LoraParams& p, int rank, int num_sms, cudaStream_t stream)
 size_t lora_workspace_bytes(int n, int rank) { return (static_cast<size_t>(rank) + 1) * n * sizeof(float); }
 
 int launch_lora_add(const LoraArgs& a, cudaStream_t stream) {
-  if (a.n < 0 || a.groups < 1 || a.groups > 1024 || a.K < 8 || a.K % 8 != 0 || a.N < 8 || a.N % 8 != 0) return kErrInvalid;
+  if (a.n < 0 || a.n > 0x7fffffff - 4096 || a.groups < 1 || a.groups > 1024 || a.K < 8 || a.K % 8 != 0 || a.N < 8 || a.N % 8 != 0) return kErrInvalid;
   if (a.fmt != kF16 && a.fmt != kBF16) return kErrInvalid;
   if (a.n == 0) return kOk;
   if (!a.y || !a.x || !a.a || !a.b || !a.scales || !a.out || !a.offsets || !a.rows || !a.slots || !a.workspace) return kErrInvalid;

@@ -28,6 +28,7 @@ namespace sfb200 {
 namespace {
 
 constexpr int kThreads = 512, kWarps = kThreads / 32, kMaxBlocks = 128, kMaxGroups = 1024;
+constexpr int kMaxEntries = 0x7fffffff - 4096;      // the strides of the loops stay inside 32 bits
 
 struct GroupParams {
   const int* ids;      // [n]: the caller's, or the experts that the router wrote
@@ -233,7 +234,7 @@ __global__ void __launch_bounds__(group_threads<NL, ONE>()) group_kernel(const R
   const int end = begin64 + p.chunk < p.n ? begin + p.chunk : p.n;
   if (NL > 0) {
     const int t0 = blockIdx.x * r.tokens_per_block;
-    const int t1 = t0 + r.tokens_per_block < r.tokens ? t0 + r.tokens_per_block : r.tokens;
+    const int t1 = r.tokens - t0 > r.tokens_per_block ? t0 + r.tokens_per_block : r.tokens;
     route_tokens<NL == 0 ? 1 : NL, NL == 32 ? 1 : 2>(r, t0, t1);
     __syncthreads();
   }
@@ -300,7 +301,7 @@ int launch_group(const RouteParams& r, const GroupParams& p, int blocks, cudaStr
 size_t group_workspace_bytes(int groups) { return static_cast<size_t>(kMaxBlocks) * groups * sizeof(int); }
 
 int launch_group_rows(const GroupArgs& a, cudaStream_t stream) {
-  if (a.n < 0 || a.groups < 1 || a.groups > kMaxGroups || a.per_row < 1 || !a.offsets) return kErrInvalid;
+  if (a.n < 0 || a.n > kMaxEntries || a.groups < 1 || a.groups > kMaxGroups || a.per_row < 1 || !a.offsets) return kErrInvalid;
   if (a.n > 0 && (!a.ids || !a.rows || !a.slots)) return kErrInvalid;
   GroupParams p{a.ids, a.n, a.groups, a.per_row, 0, static_cast<int*>(a.workspace), a.offsets, a.rows, a.slots};
   // one block to 4096 entries: eight rounds of 512 cost less than a second launch
@@ -314,7 +315,7 @@ int launch_moe_route(const RouteArgs& a, cudaStream_t stream) {
   if (a.tokens < 0 || a.experts < 1 || a.experts > kMaxGroups || a.top_k < 1 || a.top_k > 32 || a.top_k > a.experts) return kErrInvalid;
   if (a.dtype < 0 || a.dtype > 2 || a.ld < a.experts || !a.offsets) return kErrInvalid;
   if (a.tokens > 0 && (!a.logits || !a.weights || !a.chosen || !a.rows || !a.slots)) return kErrInvalid;
-  if (static_cast<int64_t>(a.tokens) * a.top_k > 0x7fffffffll - kThreads) return kErrInvalid;
+  if (static_cast<int64_t>(a.tokens) * a.top_k > kMaxEntries) return kErrInvalid;
   const int n = a.tokens * a.top_k;
   // to 32 tokens one block (two tokens a warp) costs less than a second launch (6.2 us; 64 tokens 9.8 us, in two launches 6.6); beyond, 16 tokens a
   // block or more

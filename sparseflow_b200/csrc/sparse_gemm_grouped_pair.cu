@@ -264,10 +264,9 @@ template <class C>
 int launch_cfg(const GroupedGemmArgs& a, cudaStream_t stream) {
   const int smem = C::SMEM_BYTES + (2 * (a.experts + 1) * 4 + 15) / 16 * 16;
   if (smem > 232448) return kErrInvalid;
-  static bool attr_set[kMaxDevicesGrouped] = {};
+  static bool attr_set[kMaxDevices] = {};
   int dev = 0;
-  cudaGetDevice(&dev);
-  if (dev >= kMaxDevicesGrouped) return kErrInvalid;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= kMaxDevices) return kErrCuda;
   if (!attr_set[dev]) {
     if (cudaFuncSetAttribute(grouped_gemm_pair_kernel<C>, cudaFuncAttributeMaxDynamicSharedMemorySize, 232448) != cudaSuccess) return kErrCuda;
     attr_set[dev] = true;

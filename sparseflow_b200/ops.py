@@ -279,6 +279,7 @@ def force_token_tile(bn: int) -> None:
 # A mixture of experts over 2:4 weights, the norms between two blocks, low-rank adapters.  Group sizes stay on the device:
 # none of these calls waits for the GPU, and each can be captured into a CUDA graph.
 
+_MANY = 2 ** 31 - 4097      # rows, columns and entries that the kernels count in 32 bits
 _DT3 = {torch.float16: 0, torch.bfloat16: 1, torch.float32: 2}
 _current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
 
@@ -314,6 +315,8 @@ def _rows2d(t: torch.Tensor, name: str) -> tuple:
     """(t, row pitch in elements): 2-D with unit inner stride, rows may be strided (a view that is not so is copied)."""
     if t.dim() != 2:
         raise ValueError(f"{name} must be 2D, got {t.dim()}D")
+    if t.numel() > _MANY and max(t.shape) > _MANY:
+        raise ValueError(f"{name}: {tuple(t.shape)} is beyond 32-bit counts")
     if not t.is_contiguous() and ((t.stride(1) != 1 and t.shape[1] > 1) or (t.shape[0] > 1 and t.stride(0) < t.shape[1])):
         t = t.contiguous()
     return t, _pitch(t)
@@ -385,6 +388,8 @@ def group_rows(ids: torch.Tensor, groups: int, per_row: int = 1) -> RowGroups:
     if per_row < 1 or ids.numel() % per_row:
         raise ValueError(f"per_row {per_row} does not divide {ids.numel()} entries")
     n = ids.numel()
+    if n > _MANY:
+        raise ValueError(f"{n} entries are beyond 32-bit counts")
     L = _lib.lib()
     with _on(ids.device):
         if ids.dtype == torch.int64:

@@ -58,3 +58,9 @@ def test_calls_without_a_device_return_an_error(lib):
     assert lib.sfb200_group_rows(None, 0, 1, 1, None, None, None, None, None) != 0
     assert lib.sfb200_moe_combine(None, 8, 0, None, None, None, 0, None, 8, 0, 1, 8, 0, None) != 0
     assert lib.sfb200_grouped_scratch_bytes(100, 8, 64, 64) == 0
+
+
+def test_counts_beyond_32_bits_are_refused():
+    huge = torch.empty(1, device="meta", dtype=torch.float16).expand(2 ** 31, 1)
+    with pytest.raises(ValueError, match="32-bit"):
+        ops._rows2d(huge, "x")
