@@ -135,6 +135,19 @@ def lib() -> C.CDLL:
     return L
 
 
+_calls = None
+
+
+def calls():
+    """The entry points of the operators around the gated FFN, under their names, callable without ctypes."""
+    global _calls
+    if _calls is None:
+        lib()
+        from . import _calls as module
+        _calls = module
+    return _calls
+
+
 def check(fn: str, code: int) -> None:
     if code != 0:
         raise SfbError(fn, code)

@@ -1,4 +1,4 @@
-"""Build libsparseflow_b200.so in-tree with nvcc for sm_100a.
+"""Build libsparseflow_b200.so, and _calls.so (its Python calls without ctypes), in-tree with nvcc for sm_100a.
 
     python -m sparseflow_b200.build [--force]
 
@@ -11,10 +11,13 @@ import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(HERE, "libsparseflow_b200.so")
+CALLS_SRC = os.path.join(CSRC, "python", "calls.cpp")
+CALLS = os.path.join(HERE, "_calls.so")
 OBJ_DIR = os.path.join(HERE, "csrc", "build")
 
 NVCC_FLAGS = [
@@ -40,14 +43,14 @@ def _deps() -> list[str]:
     out = sources()
     out += [os.path.join(CSRC, f) for f in os.listdir(CSRC) if f.endswith((".h", ".cuh"))]
     out.append(os.path.join(HERE, "..", "include", "sparseflow_b200.h"))
-    out.append(os.path.abspath(__file__))
+    out += [CALLS_SRC, os.path.abspath(__file__)]
     return out
 
 
 def up_to_date() -> bool:
-    if not os.path.exists(LIB):
+    if not os.path.exists(LIB) or not os.path.exists(CALLS):
         return False
-    t = os.path.getmtime(LIB)
+    t = min(os.path.getmtime(LIB), os.path.getmtime(CALLS))
     return all(os.path.getmtime(d) <= t for d in _deps())
 
 
@@ -73,6 +76,9 @@ def build(force: bool = False, verbose: bool = False) -> str:
             raise RuntimeError(f"nvcc failed on {src}")
     cmd = [nvcc, "-shared", "-o", LIB, *objs, "-gencode", "arch=compute_100a,code=sm_100a", "-ldl"]
     subprocess.run(cmd, check=True)
+    # found beside the library whatever the working directory
+    subprocess.run([nvcc, "-shared", "-cudart", "none", "-Wno-deprecated-gpu-targets", "-O2", "-std=c++17", "-Xcompiler", "-fPIC,-fvisibility=hidden", "-I", sysconfig.get_paths()["include"],
+                    CALLS_SRC, "-o", CALLS, "-L", HERE, "-lsparseflow_b200", "-Xlinker", "-rpath,$ORIGIN"], check=True)
     return LIB
 
 

@@ -338,6 +338,11 @@ def _pitch(t: torch.Tensor) -> int:
     return t.stride(0) if t.size(0) > 1 else t.size(1)
 
 
+def _empty_like(t: torch.Tensor) -> torch.Tensor:
+    """A contiguous tensor of the same shape (for a contiguous one without the parsing of a size: half a microsecond)."""
+    return torch.empty_like(t) if t.is_contiguous() else t.new_empty(t.shape)
+
+
 def _check_out(out: torch.Tensor, like: torch.Tensor, shape: tuple, dtype: torch.dtype) -> None:
     if tuple(out.shape) != shape or out.dtype != dtype or not out.is_cuda or out.get_device() != like.get_device():
         raise ValueError(f"out must be {shape} {dtype} on {like.device}")
@@ -390,7 +395,7 @@ def group_rows(ids: torch.Tensor, groups: int, per_row: int = 1) -> RowGroups:
     n = ids.numel()
     if n > _MANY:
         raise ValueError(f"{n} entries are beyond 32-bit counts")
-    L = _lib.lib()
+    L = _lib.calls()
     with _on(ids.device):
         if ids.dtype == torch.int64:
             ids = ids.clamp(-1, groups).to(torch.int32)
@@ -420,10 +425,10 @@ def moe_route(logits: torch.Tensor, top_k: int, renormalize: bool = True) -> Rou
         raise ValueError(f"experts must be 1 .. 1024, got {E}")
     if not 1 <= top_k <= min(32, E):
         raise ValueError(f"top_k must be 1 .. {min(32, E)}, got {top_k}")
-    L = _lib.lib()
+    L = _lib.calls()
     # one allocation for the four results of n * top_k words: an allocation costs as much host time as the kernel takes
     weights, chosen, slots, rows = logits.new_empty((4, n, top_k), dtype=torch.int32).unbind(0)
-    weights, rows = weights.view(torch.float32), rows.view(-1)
+    weights, rows = weights.view(torch.float32), rows.flatten()
     offsets = logits.new_empty(E + 1, dtype=torch.int32)
     work = logits.new_empty(L.sfb200_group_workspace_bytes(E), dtype=torch.uint8) if n > 32 else None
     rc = L.sfb200_moe_route(logits.data_ptr(), ld, n, E, top_k, dt, 1 if renormalize else 0, weights.data_ptr(), chosen.data_ptr(),
@@ -530,7 +535,7 @@ def _grouped_args(x: torch.Tensor, cw: CompressedExperts, groups: RowGroups, gat
 
 
 def _grouped_scratch(x: torch.Tensor, total: int, cw: CompressedExperts) -> Optional[torch.Tensor]:
-    n = _lib.lib().sfb200_grouped_scratch_bytes(total, cw.experts, cw.rows, cw.K)
+    n = _lib.calls().sfb200_grouped_scratch_bytes(total, cw.experts, cw.rows, cw.K)
     return torch.empty(n, dtype=torch.uint8, device=x.device) if n else None
 
 
@@ -555,7 +560,7 @@ def grouped_sparse_gemm(x: torch.Tensor, cw: CompressedExperts, groups: RowGroup
     if total == 0:
         return out
     scratch = _grouped_scratch(x, total, cw) if gather else None
-    rc = _lib.lib().sfb200_grouped_sparse_gemm(x.data_ptr(), ldx, x.shape[0], groups.rows.data_ptr() if gather else None, _ptr(scratch),
+    rc = _lib.calls().sfb200_grouped_sparse_gemm(x.data_ptr(), ldx, x.shape[0], groups.rows.data_ptr() if gather else None, _ptr(scratch),
                                                cw.values.data_ptr(), cw.meta.data_ptr(), out.data_ptr(), _pitch(out), total, cw.experts, cw.rows,
                                                cw.K, _dt(x), _ptr(bias), ACT[act], groups.offsets.data_ptr(), _stream_of(x.get_device()))
     if rc:
@@ -583,7 +588,7 @@ def grouped_sparse_gemm_swiglu(x: torch.Tensor, cw_gu: CompressedExperts, groups
     if total == 0:
         return out
     scratch = _grouped_scratch(x, total, cw_gu) if gather else None
-    rc = _lib.lib().sfb200_grouped_sparse_gemm_swiglu(x.data_ptr(), ldx, x.shape[0], groups.rows.data_ptr() if gather else None,
+    rc = _lib.calls().sfb200_grouped_sparse_gemm_swiglu(x.data_ptr(), ldx, x.shape[0], groups.rows.data_ptr() if gather else None,
                                                       _ptr(scratch), cw_gu.values.data_ptr(), cw_gu.meta.data_ptr(), out.data_ptr(), _pitch(out),
                                                       total, cw_gu.experts, I, cw_gu.K, _dt(x), _ptr(gate_bias), _ptr(up_bias),
                                                       groups.offsets.data_ptr(), _stream_of(x.get_device()))
@@ -625,7 +630,7 @@ def moe_combine(y: torch.Tensor, slots: torch.Tensor, weights: torch.Tensor, res
         if residual is not None:
             _check_apart(out, residual, "residual", same=True)
         ld_out = _pitch(out)
-    rc = _lib.lib().sfb200_moe_combine(y.data_ptr(), ld_y, rows, slots.data_ptr(), weights.data_ptr(), _ptr(residual), ld_res, out.data_ptr(), ld_out,
+    rc = _lib.calls().sfb200_moe_combine(y.data_ptr(), ld_y, rows, slots.data_ptr(), weights.data_ptr(), _ptr(residual), ld_res, out.data_ptr(), ld_out,
                                        n, k, H, dt, _stream_of(dev))
     if rc:
         _lib.check("sfb200_moe_combine", rc)
@@ -697,9 +702,9 @@ def block_norm(x: torch.Tensor, y: Optional[torch.Tensor] = None, *, weight: Opt
             raise ValueError(f"gate must be [{H}], or [g, {H}] or [g, 1] with g dividing {n} rows, got {tuple(gate.shape)}")
         gate, ld_gate = _rows2d(gate, "gate")
         gate_rows, gate_cols = gate.shape
-    r = x.new_empty((n, H)) if y is not None else None
-    h = (x if y is None else y).new_empty((n, H), dtype=dtype) if weight is not None else None
-    rc = _lib.lib().sfb200_block_norm(x.data_ptr(), ld_x, _ptr(y), ld_y, _ptr(weight), _ptr(bias), _ptr(post_weight), _ptr(post_bias), _ptr(gate),
+    r = _empty_like(x) if y is not None else None
+    h = (_empty_like(x if y is None else y) if y is not None or dtype is x.dtype else x.new_empty((n, H), dtype=dtype)) if weight is not None else None
+    rc = _lib.calls().sfb200_block_norm(x.data_ptr(), ld_x, _ptr(y), ld_y, _ptr(weight), _ptr(bias), _ptr(post_weight), _ptr(post_bias), _ptr(gate),
                                       ld_gate, gate_rows, gate_cols, _ptr(r), H, _ptr(h), H, n, H, xt, yt, scale, eps,
                                       eps if post_eps is None else post_eps, 1 if kind == "layer" else 0, _stream_of(dev))
     if rc:
@@ -768,7 +773,7 @@ def lora_add(y: torch.Tensor, x: torch.Tensor, bank: LoraBank, groups: RowGroups
     _on_device_of(y, groups.offsets, "groups")
     x, ld_x = _rows16(x, "x")
     if out is None:
-        out = y.new_empty((n, bank.N))
+        out = _empty_like(y)
     else:
         _check_out(out, y, (n, bank.N), y.dtype)
         _check_apart(out, x, "x")
@@ -784,7 +789,7 @@ def lora_add(y: torch.Tensor, x: torch.Tensor, bank: LoraBank, groups: RowGroups
         ld_out = _pitch(out)
         if out.data_ptr() % 16 or ld_out % 8:
             out, ld_out = y.new_empty((n, bank.N)), bank.N
-    L = _lib.lib()
+    L = _lib.calls()
     work = y.new_empty(L.sfb200_lora_workspace_bytes(n, bank.rank), dtype=torch.uint8)
     rc = L.sfb200_lora_add(y.data_ptr(), ld_y, x.data_ptr(), ld_x, bank.a.data_ptr(), bank.b.data_ptr(), bank.scales.data_ptr(),
                            out.data_ptr(), ld_out, n, bank.adapters, bank.rank, bank.K, bank.N, _dt(y), groups.offsets.data_ptr(),

@@ -64,3 +64,23 @@ def test_counts_beyond_32_bits_are_refused():
     huge = torch.empty(1, device="meta", dtype=torch.float16).expand(2 ** 31, 1)
     with pytest.raises(ValueError, match="32-bit"):
         ops._rows2d(huge, "x")
+
+
+def test_direct_calls_convert_like_the_c_abi(lib):
+    """The module beside the library: the same functions, whole ranges checked, wrong counts and types refused."""
+    from sparseflow_b200 import _lib
+    calls = _lib.calls()
+    names = [n for n in dir(calls) if n.startswith("sfb200_")]
+    assert len(names) == 10
+    for n in names:
+        arity = len(getattr(lib, n).argtypes)
+        for count in (arity - 1, arity + 1):
+            with pytest.raises(TypeError, match=f"expected {arity} arguments"):
+                getattr(calls, n)(*[0] * count)
+    for args in ((10, 16), (2 ** 31 - 1, 128)):
+        assert calls.sfb200_lora_workspace_bytes(*args) == lib.sfb200_lora_workspace_bytes(*args)
+    for n in (2 ** 31, -2 ** 31 - 1, 2 ** 70):
+        with pytest.raises(OverflowError):
+            calls.sfb200_group_workspace_bytes(n)
+    with pytest.raises(TypeError):
+        calls.sfb200_group_workspace_bytes("8")
