@@ -12,7 +12,7 @@
 // the columns of a whole piece, 8j - m .. with m the row's offset, reads it with the neighbour's values in it (inside the tensor) and drops those; the
 // pieces at the ends of a row are stored value by value, and weights, which begin at column 0, are shifted by m from two pieces.
 // Value by value throughout where the tensors' rows do not lie alike in their pieces.
-// Measured: 4096 x 8192 (f32 stream, bf16, norm on both sides) 78 us (5.2 TB/s), 16384 x 2048 bf16 58 us (4.6 TB/s; issue-bound: 50 instructions
+// Measured: 4096 x 8192 (f32 stream, bf16, norm on both sides) 73 us replayed (5.5 TB/s; streaming stores and 256-byte prefetches: the same), 16384 x 2048 bf16 58 us (4.6 TB/s; issue-bound: 50 instructions
 // a piece), 8192 x 4097 layer norms 122 us, 24 x 4096 2.7 us (latency).
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>

