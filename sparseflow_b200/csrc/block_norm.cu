@@ -76,8 +76,8 @@ __device__ __forceinline__ void store_f(void* base, int64_t at, const float* f) 
 }
 
 // Sum over the row's threads (WARP: a warp).  `turn` alternates between two sets of parts, so that one barrier does; the parts are added by
-// every thread, in order, four per load: cheaper than a second round of shuffles.
-template <bool WARP>
+// every thread, in order, four per load: cheaper than a second round of shuffles.  PADDED: the parts of no warp are zero.
+template <bool WARP, bool PADDED>
 __device__ __forceinline__ float row_sum(float v, float (*part)[32], int& turn) {
 #pragma unroll
   for (int d = 16; d > 0; d >>= 1) v += __shfl_xor_sync(0xffffffffu, v, d);
@@ -90,7 +90,8 @@ __device__ __forceinline__ float row_sum(float v, float (*part)[32], int& turn) 
   v = 0.f;
   for (int w = 0; w < warps; w += 4) {
     const float4 q = *reinterpret_cast<const float4*>(mine + w);
-    v += q.x + (w + 1 < warps ? q.y : 0.f) + (w + 2 < warps ? q.z : 0.f) + (w + 3 < warps ? q.w : 0.f);
+    if (PADDED) v += (q.x + q.y) + (q.z + q.w);
+    else v += q.x + (w + 1 < warps ? q.y : 0.f) + (w + 2 < warps ? q.z : 0.f) + (w + 3 < warps ? q.w : 0.f);
   }
   return v;
 }
@@ -157,14 +158,17 @@ __device__ __forceinline__ void load_vector(const void* base, int64_t first, int
 __device__ __forceinline__ void copy16(uint32_t dst, const void* src, int bytes) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
 }
-template <class T, int V>
-__device__ __forceinline__ void copy_piece(uint32_t dst, const void* base, int64_t at, int64_t room) {
-  const T* src = static_cast<const T*>(base) + at;
+template <class T, int V, bool SHIFT>
+__device__ __forceinline__ void copy_piece(uint32_t dst, const T* src, int64_t room) {
 #pragma unroll
   for (int b = 0; b < V * static_cast<int>(sizeof(T)); b += 16) {
-    const int64_t left = room * static_cast<int64_t>(sizeof(T)) - b;
-    const int bytes = left >= 16 ? 16 : left > 0 ? static_cast<int>(left) : 0;
-    copy16(dst + b, bytes > 0 ? reinterpret_cast<const uint8_t*>(src) + b : base, bytes);
+    if (!SHIFT) {
+      copy16(dst + b, reinterpret_cast<const uint8_t*>(src) + b, 16);
+    } else {
+      const int64_t left = room * static_cast<int64_t>(sizeof(T)) - b;
+      const int bytes = left >= 16 ? 16 : left > 0 ? static_cast<int>(left) : 0;
+      copy16(dst + b, reinterpret_cast<const uint8_t*>(src) + (bytes > 0 ? b : 0), bytes);
+    }
   }
 }
 
@@ -176,6 +180,9 @@ template <class XT, class YT, int V, int NV, bool SHIFT, bool LAYER, bool WARP, 
 __global__ void __launch_bounds__(MAXT, MINB) block_norm_kernel(const NormParams p) {
   __shared__ __align__(16) float part[2][32];
   extern __shared__ __align__(16) uint8_t ring[];
+  if (RING)      // the parts of no warp; the first barrier of a sum comes before they are read
+    for (int i = threadIdx.x; i < 64; i += blockDim.x)
+      if ((i & 31) >= static_cast<int>(blockDim.x >> 5)) part[i >> 5][i & 31] = 0.f;
   dependency_wait();
   dependency_trigger();
   int row_i = WARP ? static_cast<int>(blockIdx.x * 8 + (threadIdx.x >> 5)) : static_cast<int>(blockIdx.x);
@@ -190,12 +197,14 @@ __global__ void __launch_bounds__(MAXT, MINB) block_norm_kernel(const NormParams
   auto fetch = [&](int r) {
     const int64_t row = r, behind = p.rows - 1 - row;
     if (r < p.rows) {
+      const XT* x = static_cast<const XT*>(p.x) + row * p.ld_x + c0;
+      const YT* y = static_cast<const YT*>(p.y) + row * p.ld_y + c0;
 #pragma unroll
       for (int n = 0; n < NV; ++n) {
         const int c = c0 + n * step;
         if (c >= p.cols) continue;
-        copy_piece<XT, V>(smem_u32(x_slot + n * blockDim.x), p.x, row * p.ld_x + c, behind * p.ld_x + p.cols - c);
-        if (p.y != nullptr) copy_piece<YT, V>(smem_u32(y_slot + n * blockDim.x), p.y, row * p.ld_y + c, behind * p.ld_y + p.cols - c);
+        copy_piece<XT, V, SHIFT>(smem_u32(x_slot + n * blockDim.x), x + n * step, behind * p.ld_x + p.cols - c);
+        if (p.y != nullptr) copy_piece<YT, V, SHIFT>(smem_u32(y_slot + n * blockDim.x), y + n * step, behind * p.ld_y + p.cols - c);
       }
     }
   };
@@ -269,7 +278,7 @@ __global__ void __launch_bounds__(MAXT, MINB) block_norm_kernel(const NormParams
         for (int n = 0; n < NV; ++n)
 #pragma unroll
           for (int i = 0; i < V; ++i) s += value(n, i);
-        mean = row_sum<WARP>(s, part, turn) * p.inv_cols;
+        mean = row_sum<WARP, RING>(s, part, turn) * p.inv_cols;
         fetch_next();
         s = 0.f;
       }
@@ -283,7 +292,7 @@ __global__ void __launch_bounds__(MAXT, MINB) block_norm_kernel(const NormParams
           s = fmaf(d, d, s);
         }
       }
-      s = row_sum<WARP>(s, part, turn);
+      s = row_sum<WARP, RING>(s, part, turn);
       fetch_next();
       return rsqrtf(s * p.inv_cols + eps);
     };
