@@ -389,7 +389,7 @@ __global__ void __launch_bounds__(MAXT, MINB) block_norm_kernel(const NormParams
 }
 
 // Rows and pieces of a row from which blocks stay: with a row or two each there is nothing to fetch ahead, and eight or more short rows per SM cover each
-// other (16384 x 1024 f32 38 us, with the ring 44; 3000 x 1001 8.6 and 10.6; 4096 x 8192 f32 83 and 78, 8192 x 4097 layer norms 160 and 122).
+// other (16384 x 1024 f32 38 us, with the ring 44; 3000 x 1001 8.6 and 10.6; 4096 x 8192 f32 83 and 73, 8192 x 4097 layer norms 160 and 122).
 constexpr int kRingRows = 4 * 148, kRingPieces = 257, kRingSizes = 17;
 
 template <class Kernel>

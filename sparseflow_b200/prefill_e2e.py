@@ -228,6 +228,9 @@ def run(layers=4, hidden=4096, inter=11008, heads=32, batch=2, seq=2048, dtype="
     out = model(ids)
     err = (out.float() - ref_out.float()).abs().max().item() / ref_out.float().abs().max().item()
     res["sparse_vs_pruned_dense_max_err_over_max"] = err        # demo/demo_harness.py:187 metric
+    # with experts the largest error is that of tokens whose second expert changes: near-ties of a router behind layers that round differently
+    per_token = (out.float() - ref_out.float()).abs().flatten(0, -2).amax(-1)
+    res["sparse_vs_pruned_dense_median_token_err_over_max"] = per_token.median().item() / ref_out.float().abs().max().item()
     arm("sparse_mlp")
     if attention:
         res["attn_linears_replaced"] = sparsify_attention(model, policy)
@@ -269,7 +272,8 @@ def main():
               f"{v['tokens_per_s']:.0f} tok/s")
     print(f"Speedup (sparse vs pruned-dense): {r['speedup_sparse_vs_pruned_dense']:.2f}x   "
           f"(sparse vs dense): {r['speedup_sparse_vs_dense']:.2f}x   MLP alone: {r['mlp_speedup']:.2f}x   "
-          f"max err / max: {r['sparse_vs_pruned_dense_max_err_over_max']:.2e}")
+          f"max err / max: {r['sparse_vs_pruned_dense_max_err_over_max']:.2e}   "
+          f"median over tokens: {r['sparse_vs_pruned_dense_median_token_err_over_max']:.2e}")
     if a.json:
         with open(a.json, "w") as f:
             json.dump(r, f, indent=1)
