@@ -93,10 +93,18 @@ def is_moe(module: nn.Module) -> bool:
 
 def make_sparseflow_moe(module: nn.Module, top_k: Optional[int] = None, renormalize: Optional[bool] = None) -> SparseFlowMoE:
     """From a module with a router ``gate`` (``nn.Linear``) and a list ``experts`` of gated MLPs (``gate_proj / up_proj / down_proj`` or
-    ``w1 / w3 / w2``).  ``top_k`` and ``renormalize`` default to the module's ``top_k`` and ``norm_topk_prob`` (True without one)."""
+    ``w1 / w3 / w2``), and no other parameters.  ``top_k`` and ``renormalize`` default to the module's ``top_k`` and ``norm_topk_prob`` (True without one)."""
     from .surgery import _get_mlp_projections
     if not is_moe(module):
         raise RuntimeError(f"Unsupported MoE layout: {type(module)}")
+    read = {id(p) for part in (module.gate, *module.experts) for p in part.parameters()}
+    others = [name for name, p in module.named_parameters() if id(p) not in read]
+    if others:      # an expert that every token takes, a gate on it: leaving them out would change the function
+        raise RuntimeError(f"Unsupported MoE layout: {type(module)} has {others} beside its router and experts")
+    for e in module.experts:
+        act = getattr(e, "act_fn", None)
+        if act is not None and not any(n in getattr(act, "__name__", type(act).__name__).lower() for n in ("silu", "swish")):
+            raise RuntimeError(f"Unsupported MoE layout: experts with {act}, SiLU is what the products apply")
     if top_k is None:
         top_k = getattr(module, "top_k", None)
         if top_k is None:

@@ -84,3 +84,31 @@ def test_direct_calls_convert_like_the_c_abi(lib):
             calls.sfb200_group_workspace_bytes(n)
     with pytest.raises(TypeError):
         calls.sfb200_group_workspace_bytes("8")
+
+
+def test_layouts_that_are_not_only_router_and_experts_are_refused():
+    from torch import nn
+    from sparseflow_b200.nn.sparseflow_moe import make_sparseflow_moe
+
+    def expert(act=None):
+        m = nn.Module()
+        m.gate_proj, m.up_proj, m.down_proj = nn.Linear(64, 64, bias=False), nn.Linear(64, 64, bias=False), nn.Linear(64, 64, bias=False)
+        if act is not None:
+            m.act_fn = act
+        return m
+
+    def block(**kw):
+        m = nn.Module()
+        m.gate, m.experts, m.top_k = nn.Linear(64, 2, bias=False), nn.ModuleList([expert(**kw) for _ in range(2)]), 1
+        return m
+
+    m = block()
+    m.shared_expert = expert()
+    with pytest.raises(RuntimeError, match="shared_expert"):
+        make_sparseflow_moe(m)
+    for act in (nn.GELU(), nn.functional.relu):
+        with pytest.raises(RuntimeError, match="SiLU"):
+            make_sparseflow_moe(block(act=act))
+    for act in (None, nn.SiLU(), nn.functional.silu):
+        with pytest.raises(ValueError, match="CUDA"):      # accepted: the weights are what is refused here
+            make_sparseflow_moe(block(act=act))
