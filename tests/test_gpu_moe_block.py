@@ -154,3 +154,62 @@ def test_prefill_command(experts):
     if not experts:      # with experts a rounding may send a token elsewhere
         # five norms, each read with three 8-bit roundings more or less (2^-8 a half step)
         assert r["fused_norms_max_err_over_max"] <= 15 * 2.0 ** -8
+
+
+def _far(g, rows, cols, dtype, pitch=2 ** 28):
+    """``rows`` rows of one buffer, so far from each other that element offsets pass 32 bits (the buffer is not written between them)."""
+    buf = torch.empty((rows - 1) * pitch + cols, dtype=dtype, device="cuda")
+    t = buf.as_strided((rows, cols), (pitch, 1))
+    t.copy_(randn(g, rows, cols, dtype=dtype))
+    return t
+
+
+def test_offsets_beyond_32_bits():
+    """Rows up to 3.2e9 elements from the first: the same results as of a dense copy, bit for bit."""
+    g, n, H, dt = gen(11), 13, 256, torch.bfloat16
+    x = _far(g, n, H, dt)
+    dense = x.contiguous()
+    ids = torch.arange(n, dtype=torch.int32, device="cuda") % 3
+    groups = ops.group_rows(ids, 3)
+    cw = ops.compress_experts(randn(g, 3, 128, H, dtype=dt))
+    for gather in (False, True):
+        assert torch.equal(ops.grouped_sparse_gemm(x, cw, groups, gather=gather), ops.grouped_sparse_gemm(dense, cw, groups, gather=gather))
+    weight = randn(g, H, dtype=dt)
+    for a, b in zip(ops.block_norm(x, dense, weight=weight), ops.block_norm(dense, dense, weight=weight)):
+        assert torch.equal(a, b)
+    slots, weights = torch.randint(0, n, (9, 4), generator=g, device="cuda").int(), torch.rand(9, 4, generator=g, device="cuda")
+    assert torch.equal(ops.moe_combine(x, slots, weights), ops.moe_combine(dense, slots, weights))
+    assert torch.equal(ops.moe_route(x, 4).experts, ops.moe_route(dense, 4).experts)
+    bank = ops.LoraBank(randn(g, 3, 16, H, dtype=dt), randn(g, 3, H, 16, dtype=dt))
+    ref = ops.lora_add(dense, dense, bank, groups)
+    assert torch.equal(ops.lora_add(x, dense, bank, groups), ref) and torch.equal(ops.lora_add(dense, x, bank, groups), ref)
+    ops.lora_add(x, dense, bank, groups, out=x)
+    assert torch.equal(x.contiguous(), ref)
+    assert ops.device_status() == 0
+
+
+def test_norms_captured_together_on_two_streams():
+    """Two graphs of norms whose blocks stay, replayed at the same time on two streams with changed inputs: nothing is shared between them."""
+    g, n, dt = gen(12), 2000, torch.bfloat16
+    sets = []
+    for H in (4096, 4099):
+        x, y, w = randn(g, n, H), randn(g, n, H, dtype=dt), randn(g, H, dtype=dt)
+        run = lambda x=x, y=y, w=w: ops.block_norm(x, y, weight=w, post_weight=w, kind="layer")  # noqa: E731
+        run()
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = run()
+        sets.append((x, y, run, graph, out, torch.cuda.Stream()))
+    for _ in range(3):
+        for x, y, *_rest in sets:
+            x.copy_(randn(g, *x.shape))
+            y.copy_(randn(g, *y.shape, dtype=dt))
+        torch.cuda.synchronize()
+        for *_rest, graph, out, stream in sets:
+            with torch.cuda.stream(stream):
+                graph.replay()
+        torch.cuda.synchronize()
+        for x, y, run, graph, out, stream in sets:
+            for a, b in zip(out, run()):
+                assert torch.equal(a, b)
