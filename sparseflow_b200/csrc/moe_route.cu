@@ -134,6 +134,7 @@ __device__ void place_chunk(const GroupParams& p, int begin, int end, int* base,
 
 __device__ __forceinline__ uint32_t order_key(float v) {
   if (!(v > -INFINITY)) return 0;                 // -inf and NaN: never chosen
+  if (v == 0.f) v = 0.f;                          // -0 and +0 are equal: a tie, one key for both
   const uint32_t u = __float_as_uint(fminf(v, FLT_MAX));
   return u ^ ((u >> 31) ? 0xffffffffu : 0x80000000u);
 }
