@@ -93,14 +93,15 @@ def is_moe(module: nn.Module) -> bool:
 
 def make_sparseflow_moe(module: nn.Module, top_k: Optional[int] = None, renormalize: Optional[bool] = None) -> SparseFlowMoE:
     """From a module with a router ``gate`` (``nn.Linear``) and a list ``experts`` of gated MLPs (``gate_proj / up_proj / down_proj`` or
-    ``w1 / w3 / w2``), and no other parameters.  ``top_k`` and ``renormalize`` default to the module's ``top_k`` and ``norm_topk_prob`` (True without one)."""
+    ``w1 / w3 / w2``), and no parameters beside those of the router and the experts' three projections.  ``top_k`` and ``renormalize`` default to the module's ``top_k`` and ``norm_topk_prob`` (True without one)."""
     from .surgery import _get_mlp_projections
     if not is_moe(module):
         raise RuntimeError(f"Unsupported MoE layout: {type(module)}")
-    read = {id(p) for part in (module.gate, *module.experts) for p in part.parameters()}
+    projections = [_get_mlp_projections(e) for e in module.experts]
+    read = {id(p) for part in (module.gate, *(m for three in projections for m in three)) for p in part.parameters()}
     others = [name for name, p in module.named_parameters() if id(p) not in read]
-    if others:      # an expert that every token takes, a gate on it: leaving them out would change the function
-        raise RuntimeError(f"Unsupported MoE layout: {type(module)} has {others} beside its router and experts")
+    if others:      # an expert that every token takes, a gate on it, a norm inside an expert: leaving them out would change the function
+        raise RuntimeError(f"Unsupported MoE layout: {type(module)} has {others} beside its router and its experts' projections")
     for e in module.experts:
         act = getattr(e, "act_fn", None)
         if act is not None and not any(n in getattr(act, "__name__", type(act).__name__).lower() for n in ("silu", "swish")):
@@ -111,7 +112,7 @@ def make_sparseflow_moe(module: nn.Module, top_k: Optional[int] = None, renormal
             raise ValueError("top_k is not given and the module has none")
     if renormalize is None:
         renormalize = bool(getattr(module, "norm_topk_prob", True))
-    gates, ups, downs = zip(*(_get_mlp_projections(e) for e in module.experts))
+    gates, ups, downs = zip(*projections)
     (g, gb), (u, ub), (d, db) = _stacked(gates, "gate"), _stacked(ups, "up"), _stacked(downs, "down")
     router = module.gate
     return SparseFlowMoE(router.weight, g, u, d, top_k, renormalize, gb, ub, db, router.bias)

@@ -1,0 +1,44 @@
+"""Which mixtures of experts the surgery takes: those whose function a router, its experts' three projections and SiLU.mul are.  Everything
+else in a block would be left out of the replacement without a word, so it is refused."""
+import pytest
+from torch import nn
+
+from sparseflow_b200.nn.sparseflow_moe import make_sparseflow_moe
+
+
+def _expert(**kw):
+    m = nn.Module()
+    for name in ("gate_proj", "up_proj", "down_proj"):
+        setattr(m, name, nn.Linear(64, 64, bias=False))
+    for name, v in kw.items():
+        setattr(m, name, v() if isinstance(v, type) else v)
+    return m
+
+
+def _block(expert=None, **kw):
+    m = nn.Module()
+    m.gate, m.experts, m.top_k = nn.Linear(64, 2, bias=False), nn.ModuleList([_expert(**(expert or {})) for _ in range(2)]), 1
+    for name, v in kw.items():
+        setattr(m, name, v)
+    return m
+
+
+def _accepted(block):
+    with pytest.raises(ValueError, match="CUDA"):      # past the layout: what is refused is that the weights are not on a GPU
+        make_sparseflow_moe(block)
+
+
+def _refused(block, match):
+    with pytest.raises(RuntimeError, match=match):
+        make_sparseflow_moe(block)
+
+
+def test_plain_block():
+    _accepted(_block())
+
+
+def test_parameters_inside_an_expert():
+    _refused(_block(expert={"ln": nn.LayerNorm(64)}), "ln.weight")
+    biased = _block()
+    biased.experts[1].scale = nn.Parameter(biased.gate.weight[0, :1].clone())
+    _refused(biased, "experts.1.scale")
