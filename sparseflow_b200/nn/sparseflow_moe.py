@@ -93,7 +93,7 @@ def is_moe(module: nn.Module) -> bool:
 
 def make_sparseflow_moe(module: nn.Module, top_k: Optional[int] = None, renormalize: Optional[bool] = None) -> SparseFlowMoE:
     """From a module with a router ``gate`` (``nn.Linear``) and a list ``experts`` of gated MLPs (``gate_proj / up_proj / down_proj`` or
-    ``w1 / w3 / w2``), and no parameters beside those of the router and the experts' three projections.  ``top_k`` and ``renormalize`` default to the module's ``top_k`` and ``norm_topk_prob`` (True without one)."""
+    ``w1 / w3 / w2``), and no parameters beside those of the router and the experts' three projections, and no buffers.  ``top_k`` and ``renormalize`` default to the module's ``top_k`` and ``norm_topk_prob`` (True without one)."""
     from .surgery import _get_mlp_projections
     if not is_moe(module):
         raise RuntimeError(f"Unsupported MoE layout: {type(module)}")
@@ -102,6 +102,9 @@ def make_sparseflow_moe(module: nn.Module, top_k: Optional[int] = None, renormal
     others = [name for name, p in module.named_parameters() if id(p) not in read]
     if others:      # an expert that every token takes, a gate on it, a norm inside an expert: leaving them out would change the function
         raise RuntimeError(f"Unsupported MoE layout: {type(module)} has {others} beside its router and its experts' projections")
+    buffers = [name for name, _ in module.named_buffers()]
+    if buffers:     # a bias on the router's choice, say: what a buffer does to the result cannot be seen from here
+        raise RuntimeError(f"Unsupported MoE layout: {type(module)} has the buffers {buffers}")
     for e in module.experts:
         act = getattr(e, "act_fn", None)
         if act is not None and not any(n in getattr(act, "__name__", type(act).__name__).lower() for n in ("silu", "swish")):

@@ -42,3 +42,15 @@ def test_parameters_inside_an_expert():
     biased = _block()
     biased.experts[1].scale = nn.Parameter(biased.gate.weight[0, :1].clone())
     _refused(biased, "experts.1.scale")
+
+
+def test_buffers():
+    shifted = _block()
+    shifted.register_buffer("e_score_correction_bias", shifted.gate.weight.detach()[:, 0].clone())
+    _refused(shifted, "e_score_correction_bias")
+    shifted = _block()
+    shifted.register_buffer("shift", shifted.gate.weight.detach()[:, 0].clone(), persistent=False)
+    _refused(shifted, "shift")
+    scaled = _block()
+    scaled.experts[0].register_buffer("scale", scaled.gate.weight.detach()[0, :1].clone())
+    _refused(scaled, "experts.0.scale")
