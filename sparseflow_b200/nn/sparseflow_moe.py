@@ -91,6 +91,12 @@ def is_moe(module: nn.Module) -> bool:
     return isinstance(getattr(module, "gate", None), nn.Linear) and hasattr(module, "experts") and len(module.experts) > 0
 
 
+def _is_silu(act) -> bool:
+    """SiLU itself, torch's or the module of this name that model libraries have: a name that only contains "silu" or "swish" may be a
+    relative of it (Hardswish, a Swish with a slope)."""
+    return act is F.silu or type(act) is nn.SiLU or type(act).__name__ == "SiLUActivation"
+
+
 def make_sparseflow_moe(module: nn.Module, top_k: Optional[int] = None, renormalize: Optional[bool] = None) -> SparseFlowMoE:
     """From a module with a router ``gate`` (``nn.Linear``) and a list ``experts`` of gated MLPs (``gate_proj / up_proj / down_proj`` or
     ``w1 / w3 / w2``), and no parameters beside those of the router and the experts' three projections, and no buffers.  ``top_k`` and ``renormalize`` default to the module's ``top_k`` and ``norm_topk_prob`` (True without one)."""
@@ -107,7 +113,7 @@ def make_sparseflow_moe(module: nn.Module, top_k: Optional[int] = None, renormal
         raise RuntimeError(f"Unsupported MoE layout: {type(module)} has the buffers {buffers}")
     for e in module.experts:
         act = getattr(e, "act_fn", None)
-        if act is not None and not any(n in getattr(act, "__name__", type(act).__name__).lower() for n in ("silu", "swish")):
+        if act is not None and not _is_silu(act):
             raise RuntimeError(f"Unsupported MoE layout: experts with {act}, SiLU is what the products apply")
     if top_k is None:
         top_k = getattr(module, "top_k", None)

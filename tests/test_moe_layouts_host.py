@@ -1,6 +1,7 @@
 """Which mixtures of experts the surgery takes: those whose function a router, its experts' three projections and SiLU.mul are.  Everything
 else in a block would be left out of the replacement without a word, so it is refused."""
 import pytest
+import torch.nn.functional as F
 from torch import nn
 
 from sparseflow_b200.nn.sparseflow_moe import make_sparseflow_moe
@@ -54,3 +55,23 @@ def test_buffers():
     scaled = _block()
     scaled.experts[0].register_buffer("scale", scaled.gate.weight.detach()[0, :1].clone())
     _refused(scaled, "experts.0.scale")
+
+
+class _SwishWithASlope(nn.Module):
+    def forward(self, x):
+        return x * (1.702 * x).sigmoid()
+
+
+@pytest.mark.parametrize("act", [nn.Hardswish(), F.hardswish, _SwishWithASlope(), nn.GELU(), F.gelu])
+def test_relatives_of_silu(act):
+    _refused(_block(expert={"act_fn": act}), "SiLU")
+
+
+class SiLUActivation(nn.Module):
+    def forward(self, x):
+        return F.silu(x)
+
+
+@pytest.mark.parametrize("act", [nn.SiLU(), nn.SiLU(inplace=True), F.silu, SiLUActivation()])
+def test_silu_itself(act):
+    _accepted(_block(expert={"act_fn": act}))
