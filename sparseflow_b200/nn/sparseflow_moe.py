@@ -97,6 +97,19 @@ def _is_silu(act) -> bool:
     return act is F.silu or type(act) is nn.SiLU or type(act).__name__ == "SiLUActivation"
 
 
+def _beside(module: nn.Module, read):
+    """(name, what) a module can apply beside its children in ``read``, under whatever name: other children, functions, names of functions
+    ("act", "hidden_act", ...).  Not what changes nothing: Identity, and Dropout, which inference does not run."""
+    for name, m in module.named_children():
+        if not any(m is r for r in read) and not isinstance(m, (nn.Identity, nn.Dropout)):
+            yield name, m
+    for name, v in vars(module).items():
+        if callable(v):
+            yield name, v
+        elif "act" in name.lower() and isinstance(v, str):
+            yield name, F.silu if v.lower() in ("silu", "swish") else v
+
+
 def make_sparseflow_moe(module: nn.Module, top_k: Optional[int] = None, renormalize: Optional[bool] = None) -> SparseFlowMoE:
     """From a module with a router ``gate`` (``nn.Linear``) and a list ``experts`` of gated MLPs (``gate_proj / up_proj / down_proj`` or
     ``w1 / w3 / w2``), and no parameters beside those of the router and the experts' three projections, and no buffers.  ``top_k`` and ``renormalize`` default to the module's ``top_k`` and ``norm_topk_prob`` (True without one)."""
@@ -111,10 +124,10 @@ def make_sparseflow_moe(module: nn.Module, top_k: Optional[int] = None, renormal
     buffers = [name for name, _ in module.named_buffers()]
     if buffers:     # a bias on the router's choice, say: what a buffer does to the result cannot be seen from here
         raise RuntimeError(f"Unsupported MoE layout: {type(module)} has the buffers {buffers}")
-    for e in module.experts:
-        act = getattr(e, "act_fn", None)
-        if act is not None and not _is_silu(act):
-            raise RuntimeError(f"Unsupported MoE layout: experts with {act}, SiLU is what the products apply")
+    for e, three in zip(module.experts, projections):
+        for name, act in _beside(e, three):
+            if not _is_silu(act):
+                raise RuntimeError(f"Unsupported MoE layout: experts with {name} = {act}, SiLU is what the products apply")
     if top_k is None:
         top_k = getattr(module, "top_k", None)
         if top_k is None:

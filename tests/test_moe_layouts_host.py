@@ -75,3 +75,25 @@ class SiLUActivation(nn.Module):
 @pytest.mark.parametrize("act", [nn.SiLU(), nn.SiLU(inplace=True), F.silu, SiLUActivation()])
 def test_silu_itself(act):
     _accepted(_block(expert={"act_fn": act}))
+
+
+@pytest.mark.parametrize("name", ["act", "activation", "activation_fn", "hidden_act", "nonlinearity"])
+def test_activations_under_other_names(name):
+    for act in (nn.GELU(), nn.functional.relu, lambda x: x):
+        _refused(_block(expert={name: act}), f"{name}.*SiLU")
+    for act in (nn.SiLU(), F.silu):
+        _accepted(_block(expert={name: act}))
+
+
+def test_activations_by_name():
+    for name in ("hidden_act", "activation", "act"):
+        _refused(_block(expert={name: "gelu"}), f"{name}.*SiLU")
+        _accepted(_block(expert={name: "silu"}))
+
+
+def test_what_an_expert_does_beside_its_products():
+    _refused(_block(expert={"norm": nn.LayerNorm(64, elementwise_affine=False)}), "norm")
+    patched = _block()
+    patched.experts[1].forward = lambda x: 2 * x
+    _refused(patched, "forward")
+    _accepted(_block(expert={"drop": nn.Dropout(0.1), "nothing": nn.Identity()}))
