@@ -94,6 +94,8 @@ def is_moe(module: nn.Module) -> bool:
 def _is_silu(act) -> bool:
     """SiLU itself, torch's or the module of this name that model libraries have: a name that only contains "silu" or "swish" may be a
     relative of it (Hardswish, a Swish with a slope)."""
+    if isinstance(act, str):
+        return act.lower() in ("silu", "swish")
     return act is F.silu or type(act) is nn.SiLU or type(act).__name__ == "SiLUActivation"
 
 
@@ -107,7 +109,27 @@ def _beside(module: nn.Module, read):
         if callable(v):
             yield name, v
         elif "act" in name.lower() and isinstance(v, str):
-            yield name, F.silu if v.lower() in ("silu", "swish") else v
+            yield name, v
+
+
+def _is_routing(v) -> bool:
+    """Of what a block may apply: the softmax that gives the weights, or the name of its experts' activation."""
+    return v is F.softmax or v is torch.softmax or type(v) is nn.Softmax or (isinstance(v, str) and _is_silu(v))
+
+
+def _other_routing(module: nn.Module) -> list:
+    """Settings of a block (or of the configuration it keeps) by which it weighs or chooses its experts otherwise: a factor on the sum, another function
+    of the logits, a cap on them, a choice inside groups of experts."""
+    config = getattr(module, "config", None)
+    named = ("routed_scaling_factor", "scoring_func", "score_function", "topk_method", "n_group", "topk_group")
+    settings = {**{n: getattr(config, n) for n in named if hasattr(config, n)}, **vars(module)}
+    found = []
+    for name, v in settings.items():
+        n, number = name.lower(), isinstance(v, (int, float)) and not isinstance(v, bool)
+        if (number and ("scal" in n and v != 1 or "group" in n and v > 1 or "softcap" in n and v != 0)
+                or isinstance(v, str) and ("scor" in n and v != "softmax" or "method" in n and v != "greedy")):
+            found.append(f"{name} = {v!r}")
+    return found
 
 
 def make_sparseflow_moe(module: nn.Module, top_k: Optional[int] = None, renormalize: Optional[bool] = None) -> SparseFlowMoE:
@@ -128,6 +150,9 @@ def make_sparseflow_moe(module: nn.Module, top_k: Optional[int] = None, renormal
         for name, act in _beside(e, three):
             if not _is_silu(act):
                 raise RuntimeError(f"Unsupported MoE layout: experts with {name} = {act}, SiLU is what the products apply")
+    beside = [name for name, v in _beside(module, (module.gate, module.experts)) if not _is_routing(v)] + _other_routing(module)
+    if beside:
+        raise RuntimeError(f"Unsupported MoE layout: {type(module)} with {beside}: the weights are the softmax of the top_k logits")
     if top_k is None:
         top_k = getattr(module, "top_k", None)
         if top_k is None:

@@ -1,6 +1,9 @@
 """Which mixtures of experts the surgery takes: those whose function a router, its experts' three projections and SiLU.mul are.  Everything
 else in a block would be left out of the replacement without a word, so it is refused."""
+from types import SimpleNamespace
+
 import pytest
+import torch
 import torch.nn.functional as F
 from torch import nn
 
@@ -97,3 +100,23 @@ def test_what_an_expert_does_beside_its_products():
     patched.experts[1].forward = lambda x: 2 * x
     _refused(patched, "forward")
     _accepted(_block(expert={"drop": nn.Dropout(0.1), "nothing": nn.Identity()}))
+
+
+@pytest.mark.parametrize("setting", [{"routed_scaling_factor": 2.5}, {"router_scale": 0.5}, {"scoring_func": "sigmoid"}, {"score_function": "sigmoid"},
+                                     {"n_group": 8}, {"topk_group": 4}, {"topk_method": "noaux_tc"}, {"router_softcapping": 30.0}])
+def test_other_routing(setting):
+    (name, _), = setting.items()
+    _refused(_block(**setting), name)
+    if name not in ("router_scale", "router_softcapping"):
+        _refused(_block(config=SimpleNamespace(**setting)), name)
+
+
+def test_functions_of_the_block():
+    _refused(_block(score=torch.sigmoid), "score")
+    _refused(_block(post=nn.LayerNorm(64, elementwise_affine=False)), "post")
+    _accepted(_block(score=torch.softmax, other=F.softmax, third=nn.Softmax(-1), drop=nn.Dropout(0.1)))
+
+
+def test_settings_that_change_nothing():
+    _accepted(_block(routed_scaling_factor=1.0, scoring_func="softmax", n_group=1, topk_group=None, topk_method="greedy", norm_topk_prob=False,
+                     num_experts=2, hidden_dim=64, hidden_act="silu", jitter_noise=0.1, config=SimpleNamespace(rope_scaling_factor=8.0, n_group=1)))
