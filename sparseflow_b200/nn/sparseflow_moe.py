@@ -87,8 +87,11 @@ def _stacked(linears, what: str):
 
 
 def is_moe(module: nn.Module) -> bool:
-    """Whether a module has the layout ``make_sparseflow_moe`` reads."""
-    return isinstance(getattr(module, "gate", None), nn.Linear) and hasattr(module, "experts") and len(module.experts) > 0
+    """Whether a module has the layout ``make_sparseflow_moe`` reads: a Linear ``gate`` and a list of experts (not their number, a module that
+    holds them stacked, or a mapping)."""
+    experts = getattr(module, "experts", None)
+    return (isinstance(getattr(module, "gate", None), nn.Linear) and isinstance(experts, (nn.ModuleList, nn.Sequential, list, tuple))
+            and len(experts) > 0 and all(isinstance(e, nn.Module) for e in experts))
 
 
 def _is_silu(act) -> bool:

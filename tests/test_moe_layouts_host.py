@@ -7,7 +7,8 @@ import torch
 import torch.nn.functional as F
 from torch import nn
 
-from sparseflow_b200.nn.sparseflow_moe import make_sparseflow_moe
+from sparseflow_b200.nn import replace_llama_mlp_module
+from sparseflow_b200.nn.sparseflow_moe import is_moe, make_sparseflow_moe
 
 
 def _expert(**kw):
@@ -120,3 +121,21 @@ def test_functions_of_the_block():
 def test_settings_that_change_nothing():
     _accepted(_block(routed_scaling_factor=1.0, scoring_func="softmax", n_group=1, topk_group=None, topk_method="greedy", norm_topk_prob=False,
                      num_experts=2, hidden_dim=64, hidden_act="silu", jitter_noise=0.1, config=SimpleNamespace(rope_scaling_factor=8.0, n_group=1)))
+
+
+def _model(mlp):
+    model, layer = nn.Module(), nn.Module()
+    layer.mlp = mlp
+    model.layers = nn.ModuleList([layer])
+    return model
+
+
+@pytest.mark.parametrize("experts", [8, None, nn.Linear(64, 64), nn.ModuleList(), nn.ModuleDict({"a": nn.Linear(64, 64)}), [1, 2]])
+def test_experts_that_are_no_list(experts):
+    """Not a mixture that is read, and no other error than for every layout that the surgery does not know."""
+    m = nn.Module()
+    m.gate, m.experts = nn.Linear(64, 2, bias=False), experts
+    assert not is_moe(m)
+    for call in (lambda: make_sparseflow_moe(m), lambda: replace_llama_mlp_module(_model(m), None)):
+        with pytest.raises(RuntimeError, match="Unsupported"):
+            call()
