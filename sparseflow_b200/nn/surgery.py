@@ -4,7 +4,10 @@ Interface of the reference's ``sparseflow/nn/surgery.py:22-99`` (``replace_llama
 policy, verbose)`` -> number of layers replaced): walks ``model.model.layers`` or ``model.layers``,
 accepts the ``gate_proj/up_proj/down_proj`` and ``w1/w3/w2`` layouts, and builds the replacement from
 the layer's own weights.  ``down_mode`` is passed through (default "dense", the reference's function).
-A mixture of experts (a router ``gate`` and a list ``experts`` of such MLPs) becomes a ``SparseFlowMoE``, whose products are all sparse.
+A mixture of experts (a router ``gate`` and a list ``experts`` of such MLPs) becomes a ``SparseFlowMoE``, whose products are all sparse, the down
+projection included: with ``down_mode="dense"`` it is taken where the experts' down weights are 2:4 already, so that pruning leaves them as they
+are, and refused otherwise.  ``policy`` goes to ``SparseFlowMLP``; like its gate and up projections, those of a mixture are sparse for every
+number of tokens.
 """
 from __future__ import annotations
 
@@ -31,12 +34,21 @@ def _layers_of(model: nn.Module):
     raise RuntimeError("Could not locate transformer layers (expected model.model.layers or model.layers).")
 
 
+def _is_24(w: torch.Tensor) -> bool:
+    return w.shape[-1] % 4 == 0 and not ((w.detach().reshape(-1, 4) != 0).sum(1) > 2).any().item()
+
+
 def replace_llama_mlp_module(model: nn.Module, policy, verbose: bool = False, down_mode: str = "dense") -> int:
     replaced = 0
     for i, layer in enumerate(_layers_of(model)):
         if not hasattr(layer, "mlp"):
             continue
         if is_moe(layer.mlp):
+            if down_mode not in ("dense", "sparse"):
+                raise ValueError("down_mode must be 'dense' or 'sparse'")
+            if down_mode == "dense" and not all(_is_24(_get_mlp_projections(e)[2].weight) for e in layer.mlp.experts):
+                raise RuntimeError("Unsupported MoE layout: down_mode='dense' keeps unpruned down projections, and the experts' products are sparse: "
+                                   "pass down_mode='sparse' to prune them, or prune the weights first")
             with torch.inference_mode(False):
                 layer.mlp = make_sparseflow_moe(layer.mlp)
             replaced += 1

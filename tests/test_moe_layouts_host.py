@@ -139,3 +139,24 @@ def test_experts_that_are_no_list(experts):
     for call in (lambda: make_sparseflow_moe(m), lambda: replace_llama_mlp_module(_model(m), None)):
         with pytest.raises(RuntimeError, match="Unsupported"):
             call()
+
+
+def test_down_mode():
+    """"dense", the default, promises an unpruned down projection: a mixture keeps it only where pruning changes nothing."""
+    with pytest.raises(RuntimeError, match="down_mode"):
+        replace_llama_mlp_module(_model(_block()), None)
+    with pytest.raises(RuntimeError, match="down_mode"):
+        replace_llama_mlp_module(_model(_block()), None, down_mode="dense")
+    with pytest.raises(ValueError, match="down_mode"):
+        replace_llama_mlp_module(_model(_block()), None, down_mode="half")
+    with pytest.raises(ValueError, match="CUDA"):
+        replace_llama_mlp_module(_model(_block()), None, down_mode="sparse")
+    pruned = _block()
+    for e in pruned.experts:
+        e.down_proj.weight.data[:, 1::4] = 0
+        e.down_proj.weight.data[:, 2::4] = 0
+    with pytest.raises(ValueError, match="CUDA"):
+        replace_llama_mlp_module(_model(pruned), None)
+    pruned.experts[1].down_proj.weight.data[5, 9] = 0.5      # one group of four with three values
+    with pytest.raises(RuntimeError, match="down_mode"):
+        replace_llama_mlp_module(_model(pruned), None)
