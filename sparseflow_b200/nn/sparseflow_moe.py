@@ -142,7 +142,11 @@ def make_sparseflow_moe(module: nn.Module, top_k: Optional[int] = None, renormal
     if not is_moe(module):
         raise RuntimeError(f"Unsupported MoE layout: {type(module)}")
     projections = [_get_mlp_projections(e) for e in module.experts]
-    read = {id(p) for part in (module.gate, *(m for three in projections for m in three)) for p in part.parameters()}
+    linears = [module.gate, *(m for three in projections for m in three)]
+    for m in linears:
+        if not isinstance(m, nn.Linear):
+            raise RuntimeError(f"Unsupported MoE layout: {type(m)} as a projection, nn.Linear is what is read")
+    read = {id(p) for m in linears for p in (m.weight, m.bias)}
     others = [name for name, p in module.named_parameters() if id(p) not in read]
     if others:      # an expert that every token takes, a gate on it, a norm inside an expert: leaving them out would change the function
         raise RuntimeError(f"Unsupported MoE layout: {type(module)} has {others} beside its router and its experts' projections")

@@ -160,3 +160,22 @@ def test_down_mode():
     pruned.experts[1].down_proj.weight.data[5, 9] = 0.5      # one group of four with three values
     with pytest.raises(RuntimeError, match="down_mode"):
         replace_llama_mlp_module(_model(pruned), None)
+
+
+class _AdaptedLinear(nn.Linear):
+    def __init__(self, *args):
+        super().__init__(*args, bias=False)
+        self.lora_a, self.lora_b = nn.Linear(64, 4, bias=False), nn.Linear(4, 64, bias=False)
+
+    def forward(self, x):
+        return super().forward(x) + self.lora_b(self.lora_a(x))
+
+
+def test_projections_that_do_more_or_are_something_else():
+    _refused(_block(expert={"down_proj": _AdaptedLinear(64, 64)}), "lora_a")
+    routed = _block()
+    routed.gate.extra = nn.Parameter(routed.gate.weight.detach().clone())
+    _refused(routed, "gate.extra")
+    other = nn.Module()
+    other.weight = nn.Parameter(routed.gate.weight.detach().clone())
+    _refused(_block(expert={"up_proj": other}), "nn.Linear")
