@@ -137,7 +137,9 @@ def _other_routing(module: nn.Module) -> list:
 
 def make_sparseflow_moe(module: nn.Module, top_k: Optional[int] = None, renormalize: Optional[bool] = None) -> SparseFlowMoE:
     """From a module with a router ``gate`` (``nn.Linear``) and a list ``experts`` of gated MLPs (``gate_proj / up_proj / down_proj`` or
-    ``w1 / w3 / w2``), and no parameters beside those of the router and the experts' three projections, and no buffers.  ``top_k`` and ``renormalize`` default to the module's ``top_k`` and ``norm_topk_prob`` (True without one)."""
+    ``w1 / w3 / w2``, all ``nn.Linear``).  A block that has more, and would become another function without it, is refused: other parameters,
+    any buffer, another activation than SiLU, another way to weigh or choose the experts.  ``top_k`` and ``renormalize`` default to the module's
+    ``top_k`` and ``norm_topk_prob`` (True without one)."""
     from .surgery import _get_mlp_projections
     if not is_moe(module):
         raise RuntimeError(f"Unsupported MoE layout: {type(module)}")
@@ -147,10 +149,11 @@ def make_sparseflow_moe(module: nn.Module, top_k: Optional[int] = None, renormal
         if not isinstance(m, nn.Linear):
             raise RuntimeError(f"Unsupported MoE layout: {type(m)} as a projection, nn.Linear is what is read")
     read = {id(p) for m in linears for p in (m.weight, m.bias)}
-    others = [name for name, p in module.named_parameters() if id(p) not in read]
+    parts = (module, *module.experts)      # experts in a plain list are not the module's children
+    others = [name for part in parts for name, p in part.named_parameters() if id(p) not in read]
     if others:      # an expert that every token takes, a gate on it, a norm inside an expert: leaving them out would change the function
         raise RuntimeError(f"Unsupported MoE layout: {type(module)} has {others} beside its router and its experts' projections")
-    buffers = [name for name, _ in module.named_buffers()]
+    buffers = [name for part in parts for name, _ in part.named_buffers()]
     if buffers:     # a bias on the router's choice, say: what a buffer does to the result cannot be seen from here
         raise RuntimeError(f"Unsupported MoE layout: {type(module)} has the buffers {buffers}")
     for e, three in zip(module.experts, projections):

@@ -179,3 +179,20 @@ def test_projections_that_do_more_or_are_something_else():
     other = nn.Module()
     other.weight = nn.Parameter(routed.gate.weight.detach().clone())
     _refused(_block(expert={"up_proj": other}), "nn.Linear")
+
+
+def test_experts_in_a_plain_list():
+    """Not registered with the block: looked through all the same."""
+    def block(**kw):
+        m = _block()
+        experts = [_expert(**kw) for _ in range(2)]
+        del m.experts
+        m.experts = experts
+        return m
+
+    _accepted(block())
+    _refused(block(ln=nn.LayerNorm(64)), "ln.weight")
+    scaled = block()
+    scaled.experts[0].register_buffer("scale", scaled.gate.weight.detach()[0, :1].clone())
+    _refused(scaled, "scale")
+    _refused(block(act_fn=nn.GELU()), "SiLU")
