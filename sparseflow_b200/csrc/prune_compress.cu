@@ -364,8 +364,6 @@ int launch_prune_compress(const PruneArgs& a, cudaStream_t stream) {
                         reinterpret_cast<uintptr_t>(a.ref_codes)) % 16 == 0);
   if (vec_ok) {
     const int kpad = p.k_tiles128 * 128;
-    const int rpad = ((p.out_rows + 127) / 128) * 128;
-    dim3 grid((kpad + 511) / 512, rpad / 16);
     BlobHead head = {};
     if (a.blob_head != nullptr) {
       memcpy(head.words, a.blob_head, sizeof(head.words));
@@ -374,13 +372,27 @@ int launch_prune_compress(const PruneArgs& a, cudaStream_t stream) {
       head.pad_bytes = static_cast<int>(static_cast<uint8_t*>(a.meta) - head.pad);
       head.bad = a.bad;
       if (head.pad_bytes < 0 || head.pad_bytes >= 256) return kErrInvalid;
-      if (a.tie == kTieLow) return launch_dependent(prune_compress_kernel<kTieLow, true>, grid, 256, 0, 0, stream, p, head);
-      else return launch_dependent(prune_compress_kernel<kTieHigh, true>, grid, 256, 0, 0, stream, p, head);
-    } else if (a.tie == kTieLow) {
-      return launch_dependent(prune_compress_kernel<kTieLow, false>, grid, 256, 0, 0, stream, p, head);
-    } else {
-      return launch_dependent(prune_compress_kernel<kTieHigh, false>, grid, 256, 0, 0, stream, p, head);
     }
+    auto kernel = a.blob_head != nullptr ? (a.tie == kTieLow ? prune_compress_kernel<kTieLow, true> : prune_compress_kernel<kTieHigh, true>)
+                                         : (a.tie == kTieLow ? prune_compress_kernel<kTieLow, false> : prune_compress_kernel<kTieHigh, false>);
+    // The grid's second axis ends at 65535 groups of 16 rows: more rows (the weights of a few hundred experts) go in slabs of whole tiles, each with its
+    // own pointers.
+    constexpr int kSlabRows = 65535 / 8 * 128;
+    const int rows = p.out_rows;
+    for (int64_t r0 = 0; r0 < rows; r0 += kSlabRows) {
+      p.out_rows = rows - r0 < kSlabRows ? static_cast<int>(rows - r0) : kSlabRows;
+      const dim3 grid((kpad + 511) / 512, (p.out_rows + 127) / 128 * 8);
+      const int rc = launch_dependent(kernel, grid, 256, 0, 0, stream, p, head);
+      if (rc != kOk) return rc;
+      const size_t sources = static_cast<size_t>(a.interleave ? kSlabRows / 2 : kSlabRows) * a.ld, done = kSlabRows;
+      p.src0 += sources;
+      if (p.src1) p.src1 += sources;
+      if (p.values) p.values += done * (a.K / 2);
+      if (p.pruned) p.pruned += done * a.K;
+      if (p.ref_codes) p.ref_codes += done * (a.K / 4);
+      if (p.meta) p.meta += done / 128 * p.k_tiles128 * 512;
+    }
+    return kOk;
   } else {
     if (a.meta != nullptr || a.blob_head != nullptr) return kErrInvalid;  // tiled metadata needs K % 16 == 0 and 16-byte alignment
     if ((reinterpret_cast<uintptr_t>(a.dense) | reinterpret_cast<uintptr_t>(a.dense2)) % 8 != 0)
