@@ -280,6 +280,7 @@ def force_token_tile(bn: int) -> None:
 # none of these calls waits for the GPU, and each can be captured into a CUDA graph.
 
 _MANY = 2 ** 31 - 4097      # rows, columns and entries that the kernels count in 32 bits
+MAX_NORM_COLS = 16384       # of block_norm: a row stays in a block's registers
 _DT3 = {torch.float16: 0, torch.bfloat16: 1, torch.float32: 2}
 _current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
 
@@ -657,8 +658,8 @@ def block_norm(x: torch.Tensor, y: Optional[torch.Tensor] = None, *, weight: Opt
         raise ValueError(f"x must be float16, bfloat16 or float32, got {x.dtype}")
     x, ld_x = _rows2d(x, "x")
     n, H = x.shape
-    if not 1 <= H <= 16384:
-        raise ValueError(f"cols must be 1 .. 16384, got {H}")
+    if not 1 <= H <= MAX_NORM_COLS:
+        raise ValueError(f"cols must be 1 .. {MAX_NORM_COLS}, got {H}")
     dtype = y.dtype if y is not None else weight.dtype if weight is not None else x.dtype
     yt = _DT3.get(dtype)
     if yt is None or (dtype != x.dtype and x.dtype != torch.float32):
