@@ -201,6 +201,14 @@ def sparsify_attention(model, policy) -> int:
     return replace_llama_full(model, policy, verbose=False, dense_uses_pruned=True)
 
 
+def errors_over_max(got, ref):
+    """(largest, median over the tokens) error over the largest value.  With experts the largest is that of tokens whose second expert
+    changes: near-ties of a router behind layers that round differently."""
+    per_token = (got.float() - ref.float()).abs().flatten(0, -2).amax(-1)
+    size = ref.float().abs().max().item()
+    return per_token.max().item() / size, per_token.median().item() / size
+
+
 def run(layers=4, hidden=4096, inter=11008, heads=32, batch=2, seq=2048, dtype="bf16", iters=10, warmup=3,
         attention=True, experts=0, top_k=2) -> dict:
     td = torch.bfloat16 if dtype == "bf16" else torch.float16
@@ -227,11 +235,8 @@ def run(layers=4, hidden=4096, inter=11008, heads=32, batch=2, seq=2048, dtype="
     n = replace_llama_mlp_module(model, policy, down_mode="sparse")
     res["mlp_layers_replaced"] = n
     out = model(ids)
-    err = (out.float() - ref_out.float()).abs().max().item() / ref_out.float().abs().max().item()
-    res["sparse_vs_pruned_dense_max_err_over_max"] = err        # demo/demo_harness.py:187 metric
-    # with experts the largest error is that of tokens whose second expert changes: near-ties of a router behind layers that round differently
-    per_token = (out.float() - ref_out.float()).abs().flatten(0, -2).amax(-1)
-    res["sparse_vs_pruned_dense_median_token_err_over_max"] = per_token.median().item() / ref_out.float().abs().max().item()
+    # the largest: demo/demo_harness.py:187 metric
+    res["sparse_vs_pruned_dense_max_err_over_max"], res["sparse_vs_pruned_dense_median_token_err_over_max"] = errors_over_max(out, ref_out)
     arm("sparse_mlp")
     if attention:
         res["attn_linears_replaced"] = sparsify_attention(model, policy)
@@ -241,7 +246,7 @@ def run(layers=4, hidden=4096, inter=11008, heads=32, batch=2, seq=2048, dtype="
         before = model(ids)
         res["norms_fused"] = model.fuse_norms()
         after = model(ids)
-        res["fused_norms_max_err_over_max"] = (after.float() - before.float()).abs().max().item() / before.float().abs().max().item()
+        res["fused_norms_max_err_over_max"], res["fused_norms_median_token_err_over_max"] = errors_over_max(after, before)
         arm("fused_norms")
     a = res["arms"]
     res["speedup_sparse_vs_pruned_dense"] = a["pruned_dense"]["ms"] / a["sparse_mlp"]["ms"]
@@ -276,6 +281,9 @@ def main():
           f"(sparse vs dense): {r['speedup_sparse_vs_dense']:.2f}x   MLP alone: {r['mlp_speedup']:.2f}x   "
           f"max err / max: {r['sparse_vs_pruned_dense_max_err_over_max']:.2e}   "
           f"median over tokens: {r['sparse_vs_pruned_dense_median_token_err_over_max']:.2e}")
+    if "fused_norms" in r["arms"]:
+        print(f"Fused norms against the arm before: max err / max {r['fused_norms_max_err_over_max']:.2e}   "
+              f"median over tokens: {r['fused_norms_median_token_err_over_max']:.2e}")
     if a.json:
         with open(a.json, "w") as f:
             json.dump(r, f, indent=1)
