@@ -382,7 +382,8 @@ SFB200_API int sfb200_block_norm(const void* x, int64_t ld_x, const void* y, int
 SFB200_API size_t sfb200_lora_workspace_bytes(int n, int rank);
 /* out[t] = y[t] + scales[g] * (x[t] . A_g^T) . B_g^T for the rows of group g (grouping with per_row = 1 over n rows); rows of no
  * group: out[t] = y[t].  a [groups, rank, K], b [groups, N, rank] contiguous, rank 8, 16, 32, 64 or 128 (pad with zeros), K and N
- * multiples of 8, pitches % 8 == 0, 16-byte aligned, groups <= 1024.  out may be y. */
+ * multiples of 8, pitches % 8 == 0, 16-byte aligned, groups <= 1024.  out may be y.  Offsets and rows out of range touch nothing outside the
+ * n rows. */
 SFB200_API int sfb200_lora_add(const void* y, int64_t ld_y, const void* x, int64_t ld_x, const void* a, const void* b, const float* scales,
                                void* out, int64_t ld_out, int n, int groups, int rank, int K, int N, int dtype, const int* offsets,
                                const int* rows, const int* slots, void* workspace, void* stream);

@@ -48,6 +48,7 @@ struct LoraParams {
 };
 
 // Tile number -> its group and rows [first, first + count); false: no such tile (and first = number of tiles).  Executed by whole warps.
+// Held inside 0 .. n whatever is in memory.
 __device__ bool find_tile(const LoraParams& p, int tile, int& group, int& first, int& count) {
   const int lane = threadIdx.x & 31;
   int before = 0;
@@ -55,8 +56,8 @@ __device__ bool find_tile(const LoraParams& p, int tile, int& group, int& first,
     const int g = g0 + lane;
     int begin = 0, size = 0;
     if (g < p.groups) {
-      begin = p.offsets[g];
-      size = p.offsets[g + 1] - begin;
+      begin = min(max(p.offsets[g], 0), p.n);
+      size = min(max(p.offsets[g + 1], begin), p.n) - begin;
     }
     const int own = (size + p.tile - 1) / p.tile;
     int end = own;
@@ -82,6 +83,14 @@ __device__ bool find_tile(const LoraParams& p, int tile, int& group, int& first,
   }
   first = before;
   return false;
+}
+
+// Row of a place for reading x; one that is no row of the batch (no grouping makes such) reads another and is not stored.
+__device__ __forceinline__ int row_read(const LoraParams& p, int place) { return min(max(p.rows[place], 0), p.n - 1); }
+// Row of a place for y and out, -1 for none.
+__device__ __forceinline__ int row_written(const LoraParams& p, int place) {
+  const int row = p.rows[place];
+  return row < p.n ? row : -1;
 }
 
 __device__ __forceinline__ uint4 load16(const uint16_t* p, bool ok) {
@@ -164,7 +173,7 @@ __global__ void __launch_bounds__(kDownWarps * 32) lora_down_kernel(const LoraPa
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       const int i = m * 16 + h * 8 + g;
-      xr[m][h] = p.x + p.rows[first + (i < count ? i : 0)] * p.ld_x + 8 * q;      // rows behind the tile: its first row, not stored
+      xr[m][h] = p.x + row_read(p, first + (i < count ? i : 0)) * p.ld_x + 8 * q;      // rows behind the tile: its first row, not stored
     }
   const uint16_t* ar = p.a + (static_cast<size_t>(group) * R + g) * p.K + 8 * q;
   float acc[MF][NF][4];
@@ -241,7 +250,7 @@ __global__ void __launch_bounds__(256, 2) lora_down_tile_kernel(const LoraParams
 #pragma unroll
   for (int j = 0; j < kTileRows / 32; ++j) {
     const int i = r0 + 32 * j;
-    xr[j] = p.x + p.rows[first + (i < count ? i : 0)] * p.ld_x + 8 * piece;      // rows behind the tile: its first row, not stored
+    xr[j] = p.x + row_read(p, first + (i < count ? i : 0)) * p.ld_x + 8 * piece;      // rows behind the tile: its first row, not stored
   }
   const uint16_t* ar = p.a + (static_cast<size_t>(group) * R + r0) * p.K + 8 * piece;
   const uint32_t dst = r0 * 128 + ((piece ^ (r0 & 7)) << 4);
@@ -412,7 +421,7 @@ __global__ void __launch_bounds__(kUpWarps * 32) lora_up_kernel(const LoraParams
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, q = lane & 3;
   int64_t row[2];      // of y and out; -1 behind the tile
 #pragma unroll
-  for (int h = 0; h < 2; ++h) row[h] = h * 8 + g < count ? p.rows[first + h * 8 + g] : -1;
+  for (int h = 0; h < 2; ++h) row[h] = h * 8 + g < count ? row_written(p, first + h * 8 + g) : -1;
   uint4 yv[2];
   uint32_t bw[S::CHUNKS][4][S::WORDS];
   auto fetch = [&](int c0) {
@@ -490,8 +499,8 @@ __global__ void __launch_bounds__(kUpWarps * 32) lora_up_tile_kernel(const LoraP
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       const int i = warp * 16 * MF + m * 16 + h * 8 + g;
-      const int64_t row = i < count ? p.rows[first + i] : 0;
-      y_row[m][h] = i < count ? p.y + row * p.ld_y + 8 * q : nullptr;
+      const int64_t row = i < count ? row_written(p, first + i) : -1;
+      y_row[m][h] = row >= 0 ? p.y + row * p.ld_y + 8 * q : nullptr;
       out_row[m][h] = p.out + row * p.ld_out + 8 * q;
     }
   // Stage: 32 columns of B_g (rows of R values; from rank 64 the 64-byte halves of odd rows are exchanged, so that eight lanes read
