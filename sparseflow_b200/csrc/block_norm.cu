@@ -388,9 +388,9 @@ __global__ void __launch_bounds__(MAXT, MINB) block_norm_kernel(const NormParams
   }
 }
 
-// Rows and pieces of a row from which blocks stay: with a row or two each there is nothing to fetch ahead, and eight or more short rows per SM cover each
+// Rows per SM and pieces of a row from which blocks stay: with a row or two each there is nothing to fetch ahead, and eight or more short rows per SM cover each
 // other (16384 x 1024 f32 38 us, with the ring 44; 3000 x 1001 8.6 and 10.6; 4096 x 8192 f32 83 and 73, 8192 x 4097 layer norms 160 and 122).
-constexpr int kRingRows = 4 * 148, kRingPieces = 257, kRingSizes = 17;
+constexpr int kRingRows = 4, kRingPieces = 257, kRingSizes = 17;
 
 template <class Kernel>
 int launch_ring(Kernel kernel, const NormParams& p, int threads, int smem, bool shift, int num_sms, std::atomic<int>* known, cudaStream_t stream) {
@@ -425,7 +425,7 @@ int launch_pieces(const NormParams& p, int num_sms, cudaStream_t stream) {
     return launch_dependent(block_norm_kernel<XT, YT, 8, 1, SHIFT, LAYER, false, false, 640, 1>, p.rows, threads(1), 0, 0, stream, p);
   const int nv = pieces <= 1024 ? 2 : 4;
   const int smem = threads(nv) * nv * 8 * static_cast<int>(sizeof(XT) + sizeof(YT) * (SHIFT ? 6 : 1));
-  if (p.rows >= kRingRows && pieces >= kRingPieces && smem <= 110 * 1024) {
+  if (p.rows >= kRingRows * num_sms && pieces >= kRingPieces && smem <= 110 * 1024) {
     static std::atomic<int> known[3][kMaxDevices * kRingSizes];
     if (pieces <= 512) return launch_ring(block_norm_kernel<XT, YT, 8, 2, SHIFT, LAYER, false, true, 256, 4>, p, threads(2), smem, SHIFT, num_sms, known[0], stream);
     if (pieces <= 1024) return launch_ring(block_norm_kernel<XT, YT, 8, 2, SHIFT, LAYER, false, true, 512, 2>, p, threads(2), smem, SHIFT, num_sms, known[1], stream);
