@@ -19,7 +19,7 @@ from .. import ops
 
 
 class SparseFlowMoE(nn.Module):
-    """``router_weight`` [experts, hidden] (any float type: the router runs in it); ``gate_weight`` / ``up_weight`` [experts, intermediate,
+    """``router_weight`` [experts, hidden] (float16, bfloat16, float32 or float64: the router's product runs in it); ``gate_weight`` / ``up_weight`` [experts, intermediate,
     hidden], ``down_weight`` [experts, hidden, intermediate] float16 or bfloat16 on CUDA; biases [experts, features] or None.
     ``renormalize``: the weights of a token's experts sum to one."""
 
@@ -63,6 +63,8 @@ class SparseFlowMoE(nn.Module):
 
     def route(self, x2d: torch.Tensor) -> ops.Routing:
         logits = F.linear(x2d.to(self.router_weight.dtype), self.router_weight, self.router_bias)
+        if logits.dtype == torch.float64:      # the product was in it; the choice is among 32-bit logits
+            logits = logits.float()
         return ops.moe_route(logits, self.top_k, renormalize=self.renormalize)
 
     @torch.no_grad()
