@@ -1,6 +1,9 @@
 // Python calls of the operators around the gated FFN (include/sparseflow_b200.h, group 1b) without ctypes: eager calls of kernels of a few
 // microseconds are bound by the host, and ctypes converts 25 arguments in 2.7 us where this takes 0.2 us.  Same names, arguments in the same order;
 // pointers are ints or None.  An int that its parameter cannot hold raises OverflowError.
+//
+// Only the stable interface of CPython from 3.10 on is used, so that one build serves every interpreter that finds it in the tree.
+#define Py_LIMITED_API 0x030A0000
 #define PY_SSIZE_T_CLEAN
 #include <Python.h>
 #include <stdint.h>
