@@ -9,6 +9,7 @@ import os
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(HERE, "libsparseflow_b200.so")
+CALLS_PATH = os.path.join(HERE, "_calls.so")
 
 _lib = None
 
@@ -143,6 +144,8 @@ def calls():
     global _calls
     if _calls is None:
         lib()
+        if not os.path.exists(CALLS_PATH):
+            raise ImportError(f"{CALLS_PATH} is missing: build it with `python -m sparseflow_b200.build`, which needs Python's headers for it")
         from . import _calls as module
         _calls = module
     return _calls

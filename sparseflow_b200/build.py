@@ -3,7 +3,8 @@
     python -m sparseflow_b200.build [--force]
 
 The library is the product: every compute entry point of the package goes through it, and the
-package refuses to work without it.
+package refuses to work without it.  ``_calls.so`` needs Python's headers; where there are none the library is built
+alone, and the operators around the gated FFN, which go through that module, say what they miss.
 """
 from __future__ import annotations
 
@@ -47,10 +48,17 @@ def _deps() -> list[str]:
     return out
 
 
+def _python_include() -> str | None:
+    """The folder of Python.h, or None."""
+    path = sysconfig.get_paths()["include"]
+    return path if os.path.exists(os.path.join(path, "Python.h")) else None
+
+
 def up_to_date() -> bool:
-    if not os.path.exists(LIB) or not os.path.exists(CALLS):
+    made = [LIB, CALLS] if _python_include() else [LIB]
+    if not all(os.path.exists(f) for f in made):
         return False
-    t = min(os.path.getmtime(LIB), os.path.getmtime(CALLS))
+    t = min(os.path.getmtime(f) for f in made)
     return all(os.path.getmtime(d) <= t for d in _deps())
 
 
@@ -76,8 +84,14 @@ def build(force: bool = False, verbose: bool = False) -> str:
             raise RuntimeError(f"nvcc failed on {src}")
     cmd = [nvcc, "-shared", "-o", LIB, *objs, "-gencode", "arch=compute_100a,code=sm_100a", "-ldl"]
     subprocess.run(cmd, check=True)
+    include = _python_include()
+    if include is None:
+        if os.path.exists(CALLS):      # of another library than this one
+            os.remove(CALLS)
+        sys.stderr.write("Python.h not found: the library is built, _calls.so (calls of the operators around the gated FFN) is not\n")
+        return LIB
     # found beside the library whatever the working directory
-    subprocess.run([nvcc, "-shared", "-cudart", "none", "-Wno-deprecated-gpu-targets", "-O2", "-std=c++17", "-Xcompiler", "-fPIC,-fvisibility=hidden", "-I", sysconfig.get_paths()["include"],
+    subprocess.run([nvcc, "-shared", "-cudart", "none", "-Wno-deprecated-gpu-targets", "-O2", "-std=c++17", "-Xcompiler", "-fPIC,-fvisibility=hidden", "-I", include,
                     CALLS_SRC, "-o", CALLS, "-L", HERE, "-lsparseflow_b200", "-Xlinker", "-rpath,$ORIGIN"], check=True)
     return LIB
 
