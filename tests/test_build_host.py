@@ -29,6 +29,7 @@ def test_build_without_python_headers(monkeypatch, tmp_path, capsys):
     monkeypatch.setattr(build, "CALLS", str(tmp_path / "_calls.so"))
     monkeypatch.setattr(build, "OBJ_DIR", str(tmp_path))
     monkeypatch.setattr(build, "sources", lambda: [])
+    monkeypatch.setattr(build, "_nvcc", lambda: "nvcc")
     monkeypatch.setattr(build.subprocess, "run", lambda cmd, **kw: made.append(cmd[cmd.index("-o") + 1]))
     monkeypatch.setattr(build.sysconfig, "get_paths", lambda: {"include": str(tmp_path)})
     (tmp_path / "_calls.so").write_text("")
