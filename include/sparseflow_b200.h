@@ -342,8 +342,8 @@ SFB200_API size_t sfb200_group_workspace_bytes(int groups);
 SFB200_API int sfb200_group_rows(const int* ids, int n, int groups, int per_row, int* offsets, int* rows, int* slots,
                                  void* workspace, void* stream);
 
-/* Router: chosen[tokens, top_k] = the top_k largest logits of a token, largest first, ties to the lowest expert;
- * weights = their softmax over all experts (renormalize: over the chosen ones).  A logit of -inf or NaN is never chosen: where fewer
+/* Router: chosen[tokens, top_k] = the top_k largest logits of a token, largest first, ties (-0 and +0 are one) to the lowest
+ * expert; weights = their softmax over all experts (renormalize: over the chosen ones).  A logit of -inf or NaN is never chosen: where fewer
  * than top_k are left, chosen is -1 and the weight 0.  +inf counts as the largest finite number.  offsets, rows, slots: the
  * grouping of the entries by expert with per_row = top_k, so rows holds tokens.  dtype: sfb200_dtype, or 2 for float logits.
  * experts <= 1024, top_k <= 32 and <= experts. */
@@ -381,7 +381,7 @@ SFB200_API int sfb200_block_norm(const void* x, int64_t ld_x, const void* y, int
 
 SFB200_API size_t sfb200_lora_workspace_bytes(int n, int rank);
 /* out[t] = y[t] + scales[g] * (x[t] . A_g^T) . B_g^T for the rows of group g (grouping with per_row = 1 over n rows); rows of no
- * group: out[t] = y[t].  a [groups, rank, K], b [groups, N, rank] contiguous, rank 8, 16, 32, 64 or 128 (pad with zeros), K and N
+ * group: out[t] = y[t].  a [groups, rank, K], b [groups, N, rank] contiguous, rank 8, 16, 32, 64 or 128 (pad with zeros, which an infinity in x turns into NaN), K and N
  * multiples of 8, pitches % 8 == 0, 16-byte aligned, groups <= 1024.  out may be y.  Offsets and rows out of range touch nothing outside the
  * n rows. */
 SFB200_API int sfb200_lora_add(const void* y, int64_t ld_y, const void* x, int64_t ld_x, const void* a, const void* b, const float* scales,

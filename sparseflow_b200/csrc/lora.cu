@@ -13,9 +13,12 @@
 // lora_up deals the columns of B_g the same way, so that a lane ends up with eight consecutive outputs of a row, and begins to read everything but
 // u before it waits for lora_down: all of that was complete before lora_down began (launch.h).
 //
-// Measured: 48 rows, 48 of 64 adapters, rank 16, 4096 -> 4096 7.7 us replayed (latency: two launches); 4097 rows, 8 adapters, rank 64,
-// 4096 -> 11008 59 us replayed (lora_down 18, lora_up 46 when profiled one by one: tensor pipe 20 and 42 % of cycles, DRAM 21 and 38 %: latency of the loads
+// Measured: 48 rows, 48 of 64 adapters, rank 16, 4096 -> 4096 8.0 us replayed (latency: two launches); 4097 rows, 8 adapters, rank 64,
+// 4096 -> 11008 68-70 us among other calls, 76 replayed in a row (lora_down 18, lora_up 46 when profiled one by one: tensor pipe 20 and 42 % of cycles, DRAM 21 and 38 %: latency of the loads
 // in front of each tile, and the issue of hi and lo products, about 14 us).
+//
+// Tiles of 128 or 16 rows are chosen by the rows per resident adapter, not per used one: the host does not know which are used.  A long prompt of one
+// request beside a bank of many runs the 16-row form, which reads its adapter once per 16 rows.
 //
 // Rounding: u is needed as a 16-bit operand; a single rounding of it would put an error of half a step of the 16-bit type on the added
 // term, so it enters as hi + lo (two instructions; what is lost is a quarter step squared).  f16: the row of u is scaled by

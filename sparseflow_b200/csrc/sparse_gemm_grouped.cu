@@ -13,6 +13,10 @@
 //
 // One persistent CTA per SM, 6 warps: warp 0 = TMA producer, warp 1 = MMA issuer and tensor-memory owner, warps 2..5 = drain
 // (tensor memory -> registers -> 16-token staging tile -> 16-byte stores, rolled over 16-column chunks).
+// Rounding: one rounding of the result.  The sums over K are 32-bit in tensor memory; the tensor cores add with an error of 2.1e-6 of the
+// result's norm at K 4096 and 6.0e-6 at 11008 (32-bit FMA chains 0.4e-6 and 0.7e-6), which moves 1 to 3 of a thousand bf16 results to a neighbouring value and
+// leaves their error against 64 bits as it was (1.64e-3 of the norm, the rounding's own).  SiLU through the fast exponential and division: of 88064
+// results of the first call below none differed from those of a 64-bit SiLU on the same sums.
 // Bound by HBM: every chosen expert's weights once.  Measured: one token of 2 experts, 22016 x 4096 37 us (5.4 TB/s); 64 tokens of 6 of
 // 64 experts, 2048 x 1408 36 us (5.8 TB/s); ncu: DRAM 61 and 68 % of peak cycles, tensor pipe 3 %.
 #include <cuda.h>

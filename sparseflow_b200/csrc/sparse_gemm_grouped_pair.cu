@@ -5,9 +5,11 @@
 //   * each CTA of the pair fetches half of the token tile, in boxes of 32 or 40 rows, or four rows per lane of several gathering warps
 //     through the grouping, where that is estimated cheaper than a permuted copy in front (plan_grouped);
 //   * two accumulator sets (256-row tiles): the drain of a tile hides behind the K loop of the next.
-// Bound by the power limit under steady load, at full clock by the K step's shared-memory traffic and the drain.  Measured: 4096 tokens, 4 of 32
-// experts, 2816 x 2048: 94 us alone at full clock (tensor pipe 53 % of cycles, L2 59 %), under load 122 us, with the tokens gathered 130-137 us;
-// 1001 tokens, 2 of 8 experts, 4096 x 11008: 127 us alone (DRAM 47 %, tensor pipe 38 %), under load 140-148 us.
+// Bound by the tiles first: a token tile ends at 240, so an expert of 250 tokens runs every weight tile through shared memory twice, with half-filled
+// instructions; the last pass over the pairs is partly empty; a K loop of few steps leaves the drain's share large.  Clocks under steady load come on
+// top.  Measured: 4096 tokens, 4 of 32 experts, 2816 x 2048 (16 K steps per tile): 94 us alone at full clock (tensor pipe 53 % of cycles, L2 59 %), under load
+// 122 us, with the tokens gathered 130-142 us; 1001 tokens, 2 of 8 experts, 4096 x 11008 (about 300 tiles on 74 pairs): 127 us alone (DRAM 47 %, tensor pipe
+// 38 %), under load 140-152 us.
 #include <cuda.h>
 #include <cuda_runtime.h>
 #include <stdint.h>

@@ -412,7 +412,7 @@ def group_rows(ids: torch.Tensor, groups: int, per_row: int = 1) -> RowGroups:
 
 @_on_own_device
 def moe_route(logits: torch.Tensor, top_k: int, renormalize: bool = True) -> Routing:
-    """Route tokens to experts: the ``top_k`` largest of ``logits[tokens, experts]`` (ties to the lowest expert), their softmax
+    """Route tokens to experts: the ``top_k`` largest of ``logits[tokens, experts]`` (ties, -0 and +0 among them, to the lowest expert), their softmax
     weights (over all experts, or with ``renormalize`` over the chosen ones), and the grouping of the tokens by expert.
 
     A logit of -inf or NaN is never chosen; a token with fewer than ``top_k`` others gets expert -1 with weight 0 there (a row of
@@ -715,7 +715,8 @@ def block_norm(x: torch.Tensor, y: Optional[torch.Tensor] = None, *, weight: Opt
 
 class LoraBank:
     """Low-rank adapters of one projection: ``a`` [adapters, rank, K], ``b`` [adapters, N, rank], ``scales`` [adapters] float32 (or one
-    number).  The rank is padded with zeros to 8, 16, 32, 64 or 128; adapters of different ranks go through ``from_adapters``."""
+    number).  The rank is padded with zeros to 8, 16, 32, 64 or 128 (a row of ``x`` with an infinity meets them and comes out NaN); adapters of different
+    ranks go through ``from_adapters``."""
     RANKS = (8, 16, 32, 64, 128)
 
     def __init__(self, a: torch.Tensor, b: torch.Tensor, scales=1.0):
