@@ -122,17 +122,21 @@ def _is_routing(v) -> bool:
     return v is F.softmax or v is torch.softmax or type(v) is nn.Softmax or (isinstance(v, str) and _is_silu(v))
 
 
-def _other_routing(module: nn.Module) -> list:
-    """Settings of a block (or of the configuration it keeps) by which it weighs or chooses its experts otherwise: a factor on the sum, another function
-    of the logits, a cap on them, a choice inside groups of experts."""
+_FACTORS, _BOUNDS = ("scal", "multiplier", "alpha", "beta"), ("softcap", "limit", "clamp", "clip", "capacity")
+
+
+def _other_settings(module: nn.Module) -> list:
+    """Settings of a block (or of the configuration it keeps) or of an expert by which it computes otherwise: a factor, a bound on values or on the
+    tokens of an expert, another function of the logits, a choice inside groups of experts."""
     config = getattr(module, "config", None)
     named = ("routed_scaling_factor", "scoring_func", "score_function", "topk_method", "n_group", "topk_group")
     settings = {**{n: getattr(config, n) for n in named if hasattr(config, n)}, **vars(module)}
     found = []
     for name, v in settings.items():
         n, number = name.lower(), isinstance(v, (int, float)) and not isinstance(v, bool)
-        if (number and ("scal" in n and v != 1 or "group" in n and v > 1 or "softcap" in n and v != 0)
-                or isinstance(v, str) and ("scor" in n and v != "softmax" or "method" in n and v != "greedy")):
+        has = lambda *words: any(w in n for w in words)  # noqa: E731
+        if (number and (has(*_FACTORS) and v != 1 or has(*_BOUNDS) and v != 0 or has("group") and v > 1)
+                or isinstance(v, str) and (has("scor") and v != "softmax" or has("method") and v != "greedy")):
             found.append(f"{name} = {v!r}")
     return found
 
@@ -162,7 +166,9 @@ def make_sparseflow_moe(module: nn.Module, top_k: Optional[int] = None, renormal
         for name, act in _beside(e, three):
             if not _is_silu(act):
                 raise RuntimeError(f"Unsupported MoE layout: experts with {name} = {act}, SiLU is what the products apply")
-    beside = [name for name, v in _beside(module, (module.gate, module.experts)) if not _is_routing(v)] + _other_routing(module)
+        if _other_settings(e):
+            raise RuntimeError(f"Unsupported MoE layout: experts with {_other_settings(e)}")
+    beside = [name for name, v in _beside(module, (module.gate, module.experts)) if not _is_routing(v)] + _other_settings(module)
     if beside:
         raise RuntimeError(f"Unsupported MoE layout: {type(module)} with {beside}: the weights are the softmax of the top_k logits")
     if top_k is None:

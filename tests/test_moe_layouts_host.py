@@ -196,3 +196,16 @@ def test_experts_in_a_plain_list():
     scaled.experts[0].register_buffer("scale", scaled.gate.weight.detach()[0, :1].clone())
     _refused(scaled, "scale")
     _refused(block(act_fn=nn.GELU()), "SiLU")
+
+
+@pytest.mark.parametrize("setting", [{"alpha": 1.702}, {"swiglu_limit": 7.0}, {"output_multiplier": 0.5}, {"clamp_value": 10}])
+def test_settings_of_an_expert(setting):
+    (name, _), = setting.items()
+    _refused(_block(expert=setting), name)
+    _refused(_block(**setting), name)
+    _accepted(_block(expert={name: None, "hidden_size": 64, "intermediate_size": 64, "config": SimpleNamespace(alpha=2.0)}))
+
+
+def test_bounds_on_the_tokens_of_an_expert():
+    _refused(_block(capacity_factor=1.25), "capacity_factor")
+    _accepted(_block(capacity_factor=None))
