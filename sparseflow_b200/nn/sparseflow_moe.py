@@ -145,7 +145,7 @@ def make_sparseflow_moe(module: nn.Module, top_k: Optional[int] = None, renormal
     """From a module with a router ``gate`` (``nn.Linear``) and a list ``experts`` of gated MLPs (``gate_proj / up_proj / down_proj`` or
     ``w1 / w3 / w2``, all ``nn.Linear``).  A block that has more, and would become another function without it, is refused: other parameters,
     any buffer, another activation than SiLU, another way to weigh or choose the experts.  ``top_k`` and ``renormalize`` default to the module's
-    ``top_k`` and ``norm_topk_prob`` (True without one)."""
+    ``top_k`` and ``norm_topk_prob`` (its configuration's where it has none, True without either)."""
     from .surgery import _get_mlp_projections
     if not is_moe(module):
         raise RuntimeError(f"Unsupported MoE layout: {type(module)}")
@@ -176,7 +176,11 @@ def make_sparseflow_moe(module: nn.Module, top_k: Optional[int] = None, renormal
         if top_k is None:
             raise ValueError("top_k is not given and the module has none")
     if renormalize is None:
-        renormalize = bool(getattr(module, "norm_topk_prob", True))
+        renormalize = getattr(module, "norm_topk_prob", getattr(getattr(module, "config", None), "norm_topk_prob", None))
+        others = [name for name, v in vars(module).items() if isinstance(v, bool) and "norm" in name.lower()]
+        if renormalize is None and others:
+            raise RuntimeError(f"Unsupported MoE layout: {type(module)} with {others}: pass renormalize")
+        renormalize = True if renormalize is None else bool(renormalize)
     gates, ups, downs = zip(*projections)
     (g, gb), (u, ub), (d, db) = _stacked(gates, "gate"), _stacked(ups, "up"), _stacked(downs, "down")
     router = module.gate

@@ -209,3 +209,17 @@ def test_settings_of_an_expert(setting):
 def test_bounds_on_the_tokens_of_an_expert():
     _refused(_block(capacity_factor=1.25), "capacity_factor")
     _accepted(_block(capacity_factor=None))
+
+
+def test_normalisation_of_the_weights(monkeypatch):
+    made = []
+    monkeypatch.setattr("sparseflow_b200.nn.sparseflow_moe.SparseFlowMoE", lambda *args: made.append(args[5]))
+    for block, want in ((_block(), True), (_block(norm_topk_prob=False), False), (_block(norm_topk_prob=True), True),
+                        (_block(config=SimpleNamespace(norm_topk_prob=False)), False),
+                        (_block(norm_topk_prob=True, config=SimpleNamespace(norm_topk_prob=False)), True)):
+        make_sparseflow_moe(block)
+        assert made.pop() is want
+    for name in ("renormalize", "normalize_weights"):      # a name that is not known is not guessed at
+        _refused(_block(**{name: False}), name)
+        make_sparseflow_moe(_block(**{name: False}), renormalize=False)
+        assert made.pop() is False
