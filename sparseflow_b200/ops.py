@@ -10,7 +10,7 @@ from __future__ import annotations
 
 import ctypes as C
 import functools
-from dataclasses import dataclass
+from dataclasses import dataclass, field
 from typing import Optional
 
 import torch
@@ -366,12 +366,14 @@ def _check_apart(out: torch.Tensor, t: torch.Tensor, name: str, same: bool = Fal
 @dataclass
 class RowGroups:
     """Entries grouped by id.  ``offsets[g]`` .. ``offsets[g + 1]`` are the places of group g; ``rows[place]`` is the row the entry
-    at a place belongs to (-1 behind the last group); ``slots[entry]`` is an entry's place (-1: of no group)."""
+    at a place belongs to (-1 behind the last group); ``slots[entry]`` is an entry's place (-1: of no group).  One that is written by hand:
+    contiguous int32 tensors of these lengths."""
     offsets: torch.Tensor
     rows: torch.Tensor
     slots: torch.Tensor
     groups: int
     per_row: int = 1
+    made_here: bool = field(default=False, repr=False, compare=False)      # by group_rows or moe_route: not looked at again
 
 
 @dataclass
@@ -381,6 +383,17 @@ class Routing:
     weights: torch.Tensor
     experts: torch.Tensor
     groups: RowGroups
+
+
+def _check_groups(t: torch.Tensor, groups: RowGroups, slots: bool) -> None:
+    """The kernels read ``groups + 1`` offsets, and a row and (``slots``) a slot per entry, as int32."""
+    if groups.made_here:
+        return _on_device_of(t, groups.offsets, "groups")
+    if groups.offsets.numel() != groups.groups + 1 or (slots and groups.slots.numel() != groups.rows.numel()):
+        raise ValueError(f"a grouping of {groups.groups} groups has {groups.groups + 1} offsets, and a slot per row")
+    for name, v in (("offsets", groups.offsets), ("rows", groups.rows)) + ((("slots", groups.slots),) if slots else ()):
+        if v.dtype != torch.int32 or not v.is_contiguous() or v.device != t.device:
+            raise ValueError(f"groups.{name} must be a contiguous int32 tensor on {t.device}, got {v.dtype} on {v.device}")
 
 
 def group_rows(ids: torch.Tensor, groups: int, per_row: int = 1) -> RowGroups:
@@ -407,7 +420,7 @@ def group_rows(ids: torch.Tensor, groups: int, per_row: int = 1) -> RowGroups:
         work = torch.empty(L.sfb200_group_workspace_bytes(groups), dtype=torch.uint8, device=ids.device) if n > 4096 else None
         rc = L.sfb200_group_rows(ids.data_ptr(), n, groups, per_row, offsets.data_ptr(), rows.data_ptr(), slots.data_ptr(), _ptr(work), _stream())
     _lib.check("sfb200_group_rows", rc)
-    return RowGroups(offsets, rows, slots, groups, per_row)
+    return RowGroups(offsets, rows, slots, groups, per_row, True)
 
 
 @_on_own_device
@@ -436,7 +449,7 @@ def moe_route(logits: torch.Tensor, top_k: int, renormalize: bool = True) -> Rou
                             offsets.data_ptr(), rows.data_ptr(), slots.data_ptr(), _ptr(work), _stream_of(logits.get_device()))
     if rc:
         _lib.check("sfb200_moe_route", rc)
-    return Routing(weights, chosen, RowGroups(offsets, rows, slots, E, top_k))
+    return Routing(weights, chosen, RowGroups(offsets, rows, slots, E, top_k, True))
 
 
 @dataclass
@@ -525,7 +538,7 @@ def _grouped_args(x: torch.Tensor, cw: CompressedExperts, groups: RowGroups, gat
     if groups.groups != cw.experts:
         raise ValueError(f"grouping has {groups.groups} groups, the weights {cw.experts} experts")
     _on_device_of(x, cw.values, "weights")
-    _on_device_of(x, groups.offsets, "groups")
+    _check_groups(x, groups, False)
     total = groups.rows.numel()
     if gather:
         if x.shape[0] * groups.per_row != total:
@@ -772,7 +785,7 @@ def lora_add(y: torch.Tensor, x: torch.Tensor, bank: LoraBank, groups: RowGroups
         raise ValueError(f"grouping must be group_rows(ids, {bank.adapters}) of {n} rows")
     _on_device_of(y, x, "x")
     _on_device_of(y, bank.a, "adapters")
-    _on_device_of(y, groups.offsets, "groups")
+    _check_groups(y, groups, True)
     x, ld_x = _rows16(x, "x")
     if out is None:
         out = _empty_like(y)
