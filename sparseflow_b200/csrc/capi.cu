@@ -26,6 +26,22 @@ namespace sfb200 {
 static DeviceState g_states[kMaxDevices];
 static std::mutex g_state_mu;
 
+// The first call on a device may be one that is being captured.  Neither the allocation nor the clearing belongs to the graph: the thread is let
+// off the capture's rule against such calls meanwhile, and the word is cleared on a stream of its own.
+static bool make_status_word(int** status) {
+  cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+  if (cudaThreadExchangeStreamCaptureMode(&mode) != cudaSuccess) return false;
+  cudaStream_t own = nullptr;
+  int* word = nullptr;
+  const bool ok = cudaStreamCreateWithFlags(&own, cudaStreamNonBlocking) == cudaSuccess && cudaMalloc(&word, 256) == cudaSuccess &&
+                  cudaMemsetAsync(word, 0, 256, own) == cudaSuccess && cudaStreamSynchronize(own) == cudaSuccess;
+  if (own) cudaStreamDestroy(own);
+  if (!ok && word) cudaFree(word);
+  cudaThreadExchangeStreamCaptureMode(&mode);
+  if (ok) *status = word;
+  return ok;
+}
+
 DeviceState* device_state(int* err) {
   int dev = -1;
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= kMaxDevices) {
@@ -50,7 +66,7 @@ DeviceState* device_state(int* err) {
     if (err) *err = kErrNotSupported;
     return nullptr;
   }
-  if (cudaMalloc(&s->status, 256) != cudaSuccess || cudaMemset(s->status, 0, 256) != cudaSuccess) {
+  if (!make_status_word(&s->status)) {
     if (err) *err = kErrOutOfMemory;
     cudaGetLastError();
     return nullptr;
